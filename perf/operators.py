@@ -176,7 +176,7 @@ def prepare(case, seed):
     op = case["op"]
     if not own:
         return s
-    smg = s["smg"] = _smg()
+    smg = _smg()
     if op == "fp8":
         s["weights"] = smg.Fp8Weights(s.pop("codes"), s.pop("scales"), case["n"], case["k"])
         s["c"] = torch.empty(case["m"], case["n"], dtype=s["a"].dtype, device=DEV)
@@ -287,7 +287,7 @@ def run(s):
     op, case = s["case"]["op"], s["case"]
     if not own:
         return {"fp8": _plain_fp8, "route": _plain_route, "experts": _plain_experts}[op](s)
-    smg = s["smg"]
+    smg = _smg()
     if op == "fp8":
         f = smg.matmul_fp8_bf16_ep if case["bf16"] else smg.matmul_fp8_ep
         return f(s["a"], s["weights"], s["c"], case["m"], s["ep"])
