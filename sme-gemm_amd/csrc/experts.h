@@ -43,17 +43,15 @@ struct ExpertPlan {
     int32_t *place;       // [assignments] the padded row, -1: no expert
     int32_t *rank;        // [assignments] the place among its expert's rows, -1
     int32_t *source;      // [max_rows] the assignment, -1: padding
-    float *weight;        // [max_rows] its weight (0: padding)
     uint32_t assignments, top_k, experts;
     uint32_t max_rows, max_tiles;  // what any choice of experts may need
 };
 enum : uint32_t { EXPERT_TILES = 0, EXPERT_ROWS = 1 };
 
 // The plan's rows times their expert's weights: with `up` the hidden values act(a W) *
-// (a up), quantized into h, else C to dst [max_rows][w.n]: f32 for bf16 calls, else f16
-// and times the assignments' weights.
+// (a up), quantized into h, else C to dst [max_rows][w.n].
 hipError_t launch_fp8_grouped(const Fp8Mat &w, const Fp8Mat *up, uint32_t act, const ExpertPlan &p, Fp8Rows a, Fp8Rows h,
-                              void *dst, bool bf16, hipStream_t s);
+                              float *dst, hipStream_t s);
 
 // out [rows][d] (16-bit, of x's type), or y (f32) += out: the weighted sum over each
 // row's experts. ids outside 0 .. experts - 1 stand for no expert.

@@ -18,7 +18,7 @@
 // What bounds it: few rows, reading the weights of the experts that are used; many
 // rows, the products. Measured (weights from memory): one row, 6 of 64 experts, 2048 to 1280
 // 14.5 us (47 MB); 37 rows, 8 of 64, 4096 to 1792 270 us (1.39 GB, 5.1 TB/s); 3001 rows, 8 of
-// 128, 2048 to 1000 345 us; 2048 rows, 2 of 8, 4096 to 14336 850 us (1.7 PFLOP/s).
+// 128, 2048 to 1000 407 us; 2048 rows, 2 of 8, 4096 to 14336 892 us (1.6 PFLOP/s).
 #include <algorithm>
 
 #include "experts.h"
@@ -471,12 +471,12 @@ __global__ void __launch_bounds__(EG_NT, 4) experts_down_token(EgArgs g) {
 }
 
 // out[r] (or y[r] +=) the weighted sum of the row's experts' parts, in the order of its
-// ids; a part's row is the assignment's, or place[assignment]. F16: parts of f16 that have
-// their weights (the grouped product's of f16 rows: 2^-12 of each part, at half the traffic
-// of f32, which for bf16 would cost a step of the result's own), else f32. A workgroup takes
-// 2048 columns of a row, a thread 8, four experts' parts in flight. VEC: whole groups of 8.
-template <bool F16, bool BF16, bool VEC>
-__global__ void __launch_bounds__(256) experts_sum(const void *part, const int32_t *place, const int32_t *ids,
+// ids; a part's row is the assignment's, or place[assignment]. Parts are f32: one may lie past
+// an f16's range, or below its steps, where the sum and y do not (f16 parts took 369 us for
+// 3001 rows, 8 of 128 experts, 407 with f32). A workgroup takes 2048 columns of a row, a
+// thread 8, four experts' parts in flight. VEC: whole groups of 8.
+template <bool BF16, bool VEC>
+__global__ void __launch_bounds__(256) experts_sum(const float *part, const int32_t *place, const int32_t *ids,
                                                    const float *weights, uint32_t top_k, uint32_t experts, uint32_t d,
                                                    uint32_t parts, uint16_t *out, float *y) {
     const uint32_t r = blockIdx.x / parts, col = (blockIdx.x % parts * 256 + threadIdx.x) * 8;
@@ -486,7 +486,6 @@ __global__ void __launch_bounds__(256) experts_sum(const void *part, const int32
     float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     for (uint32_t j0 = 0; j0 < top_k; j0 += U) {
         float w[U];
-        uint4 v[U][F16 ? 1 : 2];
         float x[U][8];
 #pragma unroll
         for (int u = 0; u < U; u++) {
@@ -494,19 +493,21 @@ __global__ void __launch_bounds__(256) experts_sum(const void *part, const int32
             const int e = j0 + u < top_k ? ids[as] : -1;
             w[u] = 0.0f;
 #pragma unroll
-            for (int c = 0; c < (F16 ? 1 : 2); c++) v[u][c] = make_uint4(0, 0, 0, 0);
-#pragma unroll
             for (int c = 0; c < 8; c++) x[u][c] = 0.0f;
             if (e < 0 || e >= (int)experts) continue;
-            if (!F16) w[u] = weights[as];
-            const size_t at = (place ? (size_t)place[as] : as) * d + col;
+            w[u] = weights[as];
+            const float *p = part + (place ? (size_t)place[as] : as) * d + col;
             if (VEC) {
-                const uint4 *p = (const uint4 *)((const uint8_t *)part + at * (F16 ? 2 : 4));
 #pragma unroll
-                for (int c = 0; c < (F16 ? 1 : 2); c++) v[u][c] = p[c];
+                for (int c = 0; c < 2; c++) {
+                    const float4 v = ((const float4 *)p)[c];
+                    x[u][4 * c] = v.x;
+                    x[u][4 * c + 1] = v.y;
+                    x[u][4 * c + 2] = v.z;
+                    x[u][4 * c + 3] = v.w;
+                }
             } else {
-                for (uint32_t c = 0; c < ne; c++)
-                    x[u][c] = F16 ? to_f32<false>(((const uint16_t *)part)[at + c]) : ((const float *)part)[at + c];
+                for (uint32_t c = 0; c < ne; c++) x[u][c] = p[c];
             }
         }
 #pragma unroll
@@ -514,15 +515,7 @@ __global__ void __launch_bounds__(256) experts_sum(const void *part, const int32
             const int e = j0 + u < top_k ? ids[(size_t)r * top_k + j0 + u] : -1;
             if (e < 0 || e >= (int)experts) continue;
 #pragma unroll
-            for (int c = 0; c < 8; c++) {
-                float f = x[u][c];
-                if (VEC) {
-                    const uint4 &q = v[u][F16 ? 0 : c / 4];
-                    const uint32_t q4[4] = {q.x, q.y, q.z, q.w};
-                    f = F16 ? to_f32<false>((uint16_t)(q4[c / 2] >> (16 * (c % 2)))) : __uint_as_float(q4[c % 4]);
-                }
-                s[c] = F16 ? s[c] + f : __builtin_fmaf(w[u], f, s[c]);
-            }
+            for (int c = 0; c < 8; c++) s[c] = __builtin_fmaf(w[u], x[u][c], s[c]);
         }
     }
     const size_t o = (size_t)r * d + col;
@@ -540,17 +533,17 @@ __global__ void __launch_bounds__(256) experts_sum(const void *part, const int32
     }
     for (uint32_t c = 0; c < ne; c++) out[o + c] = from_f32<BF16>(s[c]);
 }
-template <bool F16, bool BF16>
-hipError_t launch_sum(const ExpertCall &c, const void *part, const int32_t *place, uint32_t experts, uint32_t d,
+template <bool BF16>
+hipError_t launch_sum(const ExpertCall &c, const float *part, const int32_t *place, uint32_t experts, uint32_t d,
                       hipStream_t s) {
     const uint32_t parts = (d + 2047) / 2048;
     const dim3 grid(c.rows * parts);
     if (d % 8 == 0)
-        hipLaunchKernelGGL((experts_sum<F16, BF16, true>), grid, dim3(256), 0, s, part, place, c.ids, c.weights, c.top_k, experts, d,
+        hipLaunchKernelGGL((experts_sum<BF16, true>), grid, dim3(256), 0, s, part, place, c.ids, c.weights, c.top_k, experts, d,
                            parts, c.out, c.y);
     else
-        hipLaunchKernelGGL((experts_sum<F16, BF16, false>), grid, dim3(256), 0, s, part, place, c.ids, c.weights, c.top_k, experts,
-                           d, parts, c.out, c.y);
+        hipLaunchKernelGGL((experts_sum<BF16, false>), grid, dim3(256), 0, s, part, place, c.ids, c.weights, c.top_k, experts, d,
+                           parts, c.out, c.y);
     return hipGetLastError();
 }
 
@@ -647,14 +640,13 @@ __global__ void __launch_bounds__(PL_NT) expert_plan(const int32_t *ids, ExpertP
 // their places instead, the pieces of 16 bytes cost more than that: 48 us against 25 at
 // 3001 rows of 2048, 8 experts each.)
 template <bool BF16>
-__global__ void __launch_bounds__(256) expert_rows(const uint16_t *x, uint32_t xld, const float *weights, ExpertPlan p,
-                                                   uint32_t d, uint32_t nkb, Fp8Rows o) {
+__global__ void __launch_bounds__(256) expert_rows(const uint16_t *x, uint32_t xld, ExpertPlan p, uint32_t d, uint32_t nkb,
+                                                   Fp8Rows o) {
     const size_t w = (size_t)blockIdx.x * 4 + threadIdx.x / 64;
     const uint32_t mt = (uint32_t)(w / nkb), kb = (uint32_t)(w % nkb);
     if (mt * 16 >= p.head[EXPERT_ROWS]) return;  // whole waves, no barrier follows
     const int lane = threadIdx.x % 64, lr = lane % 16, lg = lane / 16;
     const int as = p.source[mt * 16 + lr];
-    if (kb == 0 && lg == 0) p.weight[mt * 16 + lr] = as < 0 ? 0.0f : weights[as];
     const uint16_t *xp = x + (size_t)(as < 0 ? 0 : (uint32_t)as / p.top_k) * xld;
     uint32_t a[16];
     load_x32(xp, as >= 0, kb * FP8_BLOCK + 32 * lg, d, a);
@@ -692,11 +684,10 @@ struct Layout {
     Fp8Rows x, h;
     float *hidden, *part;
     uint8_t *hq, *he;
-    void *parts;
     uint16_t *padded;
     size_t bytes;
 };
-Layout layout(const ExpertSet &e, size_t rows, size_t top_k, bool bf16, bool pads, void *scratch) {
+Layout layout(const ExpertSet &e, size_t rows, size_t top_k, bool pads, void *scratch) {
     Layout l = {};
     uint8_t *at = (uint8_t *)scratch;
     auto take = [&](size_t bytes) {
@@ -725,10 +716,9 @@ Layout layout(const ExpertSet &e, size_t rows, size_t top_k, bool bf16, bool pad
         l.p.place = (int32_t *)take(as * 4);
         l.p.rank = (int32_t *)take(as * 4);
         l.p.source = (int32_t *)take((size_t)l.p.max_rows * 4);
-        l.p.weight = (float *)take((size_t)l.p.max_rows * 4);
         l.x = Fp8Rows::at(take(Fp8Rows::bytes(l.p.max_rows, e.gate.nkb)), l.p.max_rows, e.gate.nkb);
         l.h = Fp8Rows::at(take(Fp8Rows::bytes(l.p.max_rows, e.down.nkb)), l.p.max_rows, e.down.nkb);
-        l.parts = take((size_t)l.p.max_rows * e.down.n * (bf16 ? 4 : 2));
+        l.part = (float *)take((size_t)l.p.max_rows * e.down.n * 4);
     }
     l.bytes = (size_t)(at - (uint8_t *)scratch);
     return l;
@@ -737,11 +727,11 @@ Layout layout(const ExpertSet &e, size_t rows, size_t top_k, bool bf16, bool pad
 }  // namespace
 
 size_t experts_scratch_bytes(const ExpertSet &e, const ExpertCall &c) {
-    return layout(e, c.rows, c.top_k, c.bf16, pads(e, c), nullptr).bytes;
+    return layout(e, c.rows, c.top_k, pads(e, c), nullptr).bytes;
 }
 
 hipError_t launch_experts(const ExpertSet &e, const ExpertCall &c, void *scratch, hipStream_t s) {
-    const Layout l = layout(e, c.rows, c.top_k, c.bf16, pads(e, c), scratch);
+    const Layout l = layout(e, c.rows, c.top_k, pads(e, c), scratch);
     const uint32_t d = e.gate.k, as = c.rows * c.top_k, experts = e.gate.mats, xld = l.padded ? (d + 7) / 8 * 8 : d;
     const uint16_t *x = l.padded ? l.padded : c.x;
     hipError_t err;
@@ -789,19 +779,18 @@ hipError_t launch_experts(const ExpertSet &e, const ExpertCall &c, void *scratch
         if ((err = hipGetLastError()) != hipSuccess) return err;
         hipLaunchKernelGGL(experts_down, down, dim3(EG_NT), 0, s, g);
         if ((err = hipGetLastError()) != hipSuccess) return err;
-        return c.bf16 ? launch_sum<false, true>(c, l.part, nullptr, experts, d, s) : launch_sum<false, false>(c, l.part, nullptr, experts, d, s);
+        return c.bf16 ? launch_sum<true>(c, l.part, nullptr, experts, d, s) : launch_sum<false>(c, l.part, nullptr, experts, d, s);
     }
     hipLaunchKernelGGL(expert_plan, dim3(1), dim3(PL_NT), 0, s, c.ids, l.p);
     if ((err = hipGetLastError()) != hipSuccess) return err;
     const uint32_t nkb = e.gate.nkb;
     const dim3 rows((uint32_t)(((size_t)l.p.max_rows / 16 * nkb + 3) / 4));
-    if (c.bf16) hipLaunchKernelGGL((expert_rows<true>), rows, dim3(256), 0, s, x, xld, c.weights, l.p, d, nkb, l.x);
-    else hipLaunchKernelGGL((expert_rows<false>), rows, dim3(256), 0, s, x, xld, c.weights, l.p, d, nkb, l.x);
+    if (c.bf16) hipLaunchKernelGGL((expert_rows<true>), rows, dim3(256), 0, s, x, xld, l.p, d, nkb, l.x);
+    else hipLaunchKernelGGL((expert_rows<false>), rows, dim3(256), 0, s, x, xld, l.p, d, nkb, l.x);
     if ((err = hipGetLastError()) != hipSuccess) return err;
-    if ((err = launch_fp8_grouped(e.gate, &e.up, e.act, l.p, l.x, l.h, nullptr, c.bf16, s)) != hipSuccess) return err;
-    if ((err = launch_fp8_grouped(e.down, nullptr, 0, l.p, l.h, l.h, l.parts, c.bf16, s)) != hipSuccess) return err;
-    return c.bf16 ? launch_sum<false, true>(c, l.parts, l.p.place, experts, d, s)
-                  : launch_sum<true, false>(c, l.parts, l.p.place, experts, d, s);
+    if ((err = launch_fp8_grouped(e.gate, &e.up, e.act, l.p, l.x, l.h, nullptr, s)) != hipSuccess) return err;
+    if ((err = launch_fp8_grouped(e.down, nullptr, 0, l.p, l.h, l.h, l.part, s)) != hipSuccess) return err;
+    return c.bf16 ? launch_sum<true>(c, l.part, l.p.place, experts, d, s) : launch_sum<false>(c, l.part, l.p.place, experts, d, s);
 }
 
 }  // namespace smg

@@ -38,7 +38,6 @@ struct F8Args {
     uint32_t act;
     uint8_t *hq, *he;
     uint32_t hkb;               // blocks of the hidden width
-    const float *weight;        // f16 parts: the rows' weights
 };
 
 enum F8Mode : int { F8_DENSE = 0, F8_GROUPED = 1, F8_GLU = 2 };
@@ -536,11 +535,6 @@ __device__ __forceinline__ void f8_big(const F8Args &f, const EpArgs &ep, const 
         rest(PH - 1);
         wait_vm<0>();  // the steps issued past the last
     }
-    constexpr bool WEIGHED = MODE == F8_GROUPED && !BF16;
-    float weight[PH * RT];
-    if constexpr (WEIGHED)
-#pragma unroll
-        for (int i = 0; i < PH * RT; i++) weight[i] = f.weight[min(rt0 + wr * PH * RT + i, f.mt16 - 1) * 16 + lr];
     __syncthreads();
 
     // (the thread's place, opaque: the loop then keeps none of what derives from
@@ -552,7 +546,7 @@ __device__ __forceinline__ void f8_big(const F8Args &f, const EpArgs &ep, const 
         glu_store<PH * RT, 4>(f, acc, (uint32_t *)ring, rt0, pl.rt_end, tn, wr, wc, to % 64);
         return;
     }
-    if constexpr (MODE == F8_GROUPED && BF16) {  // f32 parts, as they are
+    if constexpr (MODE == F8_GROUPED) {  // f32 parts, as they are
         float *dst = (float *)g.st.dst;
 #pragma unroll
         for (int i = 0; i < PH * RT; i++) {
@@ -572,12 +566,6 @@ __device__ __forceinline__ void f8_big(const F8Args &f, const EpArgs &ep, const 
             }
         }
         return;
-    }
-    if constexpr (WEIGHED) {  // f16 parts, with their weights: no part overflows that its row would not
-#pragma unroll
-        for (int i = 0; i < PH * RT; i++)
-#pragma unroll
-            for (int j = 0; j < 4; j++) acc[i][j] *= weight[i];
     }
     constexpr int RH = 16 * RT;  // rows of a wave's phase
     uint16_t *stg = (uint16_t *)ring;
@@ -733,11 +721,10 @@ hipError_t launch_fp8_gemm(const Fp8Mat &w, size_t m, uint16_t *dst, Fp8Rows a, 
 }
 
 hipError_t launch_fp8_grouped(const Fp8Mat &w, const Fp8Mat *up, uint32_t act, const ExpertPlan &p, Fp8Rows a, Fp8Rows h,
-                              void *dst, bool bf16, hipStream_t s) {
+                              float *dst, hipStream_t s) {
     F8Args f = {};
     DArgs &g = f.d;
-    g.st = {(uint16_t *)dst, (long)w.n, 1, 0, w.n, 0.0f, 0};
-    g.beta = 1.0f;
+    g.st.dst = (uint16_t *)dst;
     g.n = w.n;
     f.q = a.q;
     f.e = a.e;
@@ -748,7 +735,6 @@ hipError_t launch_fp8_grouped(const Fp8Mat &w, const Fp8Mat *up, uint32_t act, c
     f.nkb = w.nkb;
     f.head = p.head;
     f.tiles = p.tiles;
-    f.weight = p.weight;
     const uint32_t cols = up ? 128 : 256;
     const dim3 grid(p.max_tiles * ((w.n + cols - 1) / cols)), block(512);
     if (grid.x == 0) return hipSuccess;
@@ -761,7 +747,6 @@ hipError_t launch_fp8_grouped(const Fp8Mat &w, const Fp8Mat *up, uint32_t act, c
         f.hkb = w.n16 / 8;
     }
     if (up) hipLaunchKernelGGL((fp8_big<false, 1, F8_GLU>), grid, block, 0, s, f, EpArgs{});
-    else if (bf16) hipLaunchKernelGGL((fp8_big<true, 1, F8_GROUPED>), grid, block, 0, s, f, EpArgs{});
     else hipLaunchKernelGGL((fp8_big<false, 1, F8_GROUPED>), grid, block, 0, s, f, EpArgs{});
     return hipGetLastError();
 }
