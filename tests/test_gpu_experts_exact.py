@@ -1,9 +1,11 @@
 """The experts' products element by element, over hidden values that have no rounding of
-their own (experts_exact.py): parts of any size."""
+their own (experts_exact.py): every form's loops, decode calls of many experts, parts of
+any size, weights past 4 GB."""
 import numpy as np
 import pytest
 
 import experts_exact as exact
+import fp8_ref as ref
 from test_gpu_experts import build, run_experts
 from test_gpu_fp8 import bits, check, dev16, host16, values
 
@@ -27,6 +29,41 @@ def accumulate(e, x, ids, w, y0, bf16):
     y = torch.from_numpy(y0).cuda()
     e.accumulate(dev16(x, bf16), torch.from_numpy(ids).cuda(), torch.from_numpy(w).cuda(), y, len(x))
     return y.cpu().numpy().astype(np.float64)
+
+
+def check_both(smg, e, parts, xv, ids, w, bf16, what, y0=None):
+    """forward and accumulate."""
+    want, off, size = exact.experts(xv, parts, ids, w)
+    x = bits(xv, bf16)
+    check(values(run_experts(e, x, ids, w, bf16), bf16), want, off, bf16, what)
+    y0 = np.zeros(want.shape, np.float32) if y0 is None else y0
+    got = accumulate(e, x, ids, w, y0, bf16)
+    tol = off + 2.0 ** -24 * (np.abs(want) + 2 * np.abs(y0)) + 2.0 ** -149
+    bad = ~(np.abs(got - y0 - want) <= tol)
+    assert not bad.any(), f"{what}, accumulate: {bad.sum()} of {bad.size}, first {np.argwhere(bad)[0]}: " \
+                          f"{(got - y0)[bad][0]} for {want[bad][0]} (tol {tol[bad][0]})"
+
+
+# (rows, d, ffn, experts, top_k): one row, and past the blocks its waves hold at once (24 of
+# d, 64 of its experts' ffn); few rows, with no more assignments than experts and more, past
+# 16 blocks of either width; tiles of few and of many experts, past 64 blocks of either
+# width; the last call of the few rows' form and the first of the tiles'
+SHAPES = [(1, 64, 64, 4, 2), (1, 513, 130, 8, 6), (1, 3300, 200, 3, 2), (1, 130, 2200, 5, 4), (2, 200, 130, 64, 6),
+          (5, 136, 200, 64, 6), (8, 129, 96, 70, 8), (17, 200, 96, 6, 2), (60, 128, 384, 4, 2), (5, 2300, 140, 3, 2),
+          (20, 140, 2300, 3, 2), (300, 256, 128, 8, 2), (513, 130, 200, 3, 1), (400, 130, 96, 128, 2), (500, 40, 24, 1024, 2),
+          (200, 8400, 64, 2, 2), (200, 70, 8400, 2, 2), (48, 100, 72, 64, 8), (49, 100, 72, 64, 8), (700, 300, 260, 2, 2)]
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("rows,d,ffn,experts,top_k", SHAPES)
+def test_every_element(smg, rows, d, ffn, experts, top_k, bf16):
+    rng = np.random.default_rng(rows * 41 + d + experts)
+    parts = exact.make(rng, experts, d, ffn)
+    e = build(smg, parts, experts, d, ffn)
+    w = rng.uniform(0.1, 1, (rows, top_k)).astype(np.float32)
+    y0 = rng.standard_normal((rows, d)).astype(np.float32)
+    check_both(smg, e, parts, exact.rows_of(rng, rows, d), choose(rng, rows, experts, top_k), w, bf16,
+               f"{rows} rows, {top_k} of {experts}, {d} to {ffn}", y0)
 
 
 @pytest.mark.parametrize("bf16", [False, True])
@@ -66,3 +103,52 @@ def test_parts_that_cancel(smg, rows):
     want, off, size = exact.experts(xv, parts, ids, w)
     assert size.max() > 1e6 and np.abs(want).max() < 1e4
     check(values(run_experts(e, bits(xv, False), ids, w, False), False), want, off, False, f"{rows} rows")
+
+
+def test_a_lost_element_is_seen():
+    """Planted in the oracle's own result: an element set to zero, or to its neighbour's,
+    fails the bound nearly everywhere (its values are not all far from zero)."""
+    rng = np.random.default_rng(0)
+    for rows, d, ffn, experts, top_k in ((60, 128, 384, 4, 2), (20, 140, 2300, 3, 2)):
+        parts = exact.make(rng, experts, d, ffn)
+        want, off, _ = exact.experts(exact.rows_of(rng, rows, d), parts, choose(rng, rows, experts, top_k),
+                                     rng.uniform(0.1, 1, (rows, top_k)))
+        live = np.abs(want).sum(1) > 0
+        for other in (np.zeros_like(want), np.roll(want, 1, 1)):
+            tol = ref.half_step(True) * (np.abs(want) + off) + off
+            assert (np.abs(other - want) <= tol)[live].mean() < 0.04
+
+
+@pytest.mark.parametrize("rows", [1, 7, 500])
+def test_experts_past_4_gb(smg, rows):
+    """Offsets of more than 32 bits within a matrix: the first experts, the last and those
+    around 2^32 bytes."""
+    import torch
+    rng = np.random.default_rng(rows)
+    experts, d, ffn, k = 1024, 2048, 2100, 3
+    assert experts * d * ffn > 2 ** 32
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    small = torch.from_numpy(exact.SMALL).cuda()
+    plus, minus = (int(exact.code_of(v)) for v in (448.0, -448.0))
+
+    def codes(n, kk):
+        return torch.cat([small[torch.randint(0, 5, (64, n, kk), device="cuda", generator=g)] for _ in range(experts // 64)])
+
+    gate, up, down = codes(ffn, d), codes(ffn, d), codes(d, ffn)
+    gate[:, :, 0] = torch.where(torch.rand(experts, ffn, device="cuda", generator=g) < 0.1, minus, plus).to(torch.uint8)
+    up[:, :, 0] = 0
+    ones = torch.ones(experts, -(-ffn // 128), -(-d // 128), device="cuda")
+    low = torch.full((experts, -(-d // 128), -(-ffn // 128)), 2.0 ** -22, device="cuda")
+    at = 2 ** 32 // (d * ffn)
+    used = [0, 1, at - 1, at, at + 1, experts - 1]
+    parts = [(None, None, np.stack([ref.VALUES[m[i].cpu().numpy()] * s for i in used]))
+             for m, s in ((gate, 1.0), (up, 1.0), (down, 2.0 ** -22))]
+    e = smg.Experts(gate, ones, up, ones, down, low, experts, d, ffn)
+    del gate, up, down
+    few = choose(rng, rows, len(used), k)
+    ids = np.where((few >= 0) & (few < len(used)), np.int32(used)[np.clip(few, 0, len(used) - 1)], -1).astype(np.int32)
+    few = np.where(ids < 0, -1, few)
+    w = rng.uniform(0.1, 1, (rows, k)).astype(np.float32)
+    xv = exact.rows_of(rng, rows, d)
+    want, off, _ = exact.experts(xv, parts, few, w)
+    check(values(run_experts(e, bits(xv, True), ids, w, True), True), want, off, True, f"{rows} rows")
