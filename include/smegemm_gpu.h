@@ -527,11 +527,12 @@ int smg_route_dev(const smg_router *r, size_t rows, const void *logits, int type
  * so are the hidden values act(gate) * up (f32, never rounded before that); act is
  * EP_ACT_SILU or EP_ACT_GELU. An id outside 0 .. experts - 1 stands for no expert: it
  * adds nothing, and a row of such ids gives zeros. An expert may be named twice. The
- * experts' sums are f32 until their weighted sum is, and that is rounded once. The gate
- * and up sums of a call of up to 384 assignments, 8 an expert, lose nothing but f32's
- * roundings; those of larger ones are formed as matmul_fp8's, by matrix instructions that
- * drop what lies 2^-13 below the largest of 8 products, so that a hidden value next to the
- * border of two codes may take the other one. The same bits on every call. */
+ * experts' sums are f32 until their weighted sum is, and that is rounded once. Gate and up
+ * sums lose nothing but f32's roundings, but for smg_experts_forward of bf16 rows past 384
+ * assignments (or 8 an expert), where they are formed as matmul_fp8's, by matrix
+ * instructions that drop what lies 2^-13 below the largest of 8 products, so that a hidden
+ * value next to the border of two codes may take the other one. The same bits on every
+ * call. */
 typedef struct smg_experts smg_experts;
 int smg_experts_create(const uint8_t *gate, const float *gate_scales, const uint8_t *up, const float *up_scales,
                        const uint8_t *down, const float *down_scales, size_t experts, size_t d, size_t ffn,

@@ -49,9 +49,10 @@ struct ExpertPlan {
 enum : uint32_t { EXPERT_TILES = 0, EXPERT_ROWS = 1 };
 
 // The plan's rows times their expert's weights: with `up` the hidden values act(a W) *
-// (a up), quantized into h, else C to dst [max_rows][w.n].
+// (a up), quantized into h, else C to dst [max_rows][w.n]. exact (with `up`): sums that lose
+// nothing but f32's roundings, at the rate of f16.
 hipError_t launch_fp8_grouped(const Fp8Mat &w, const Fp8Mat *up, uint32_t act, const ExpertPlan &p, Fp8Rows a, Fp8Rows h,
-                              float *dst, hipStream_t s);
+                              float *dst, bool exact, hipStream_t s);
 
 // out [rows][d] (16-bit, of x's type), or y (f32) += out: the weighted sum over each
 // row's experts. ids outside 0 .. experts - 1 stand for no expert.

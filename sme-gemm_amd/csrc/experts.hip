@@ -18,7 +18,7 @@
 // What bounds it: few rows, reading the weights of the experts that are used; many
 // rows, the products. Measured (weights from memory): one row, 6 of 64 experts, 2048 to 1280
 // 14.5 us (47 MB); 37 rows, 8 of 64, 4096 to 1792 270 us (1.39 GB, 5.1 TB/s); 3001 rows, 8 of
-// 128, 2048 to 1000 407 us; 2048 rows, 2 of 8, 4096 to 14336 892 us (1.6 PFLOP/s).
+// 128, 2048 to 1000 532 us (f16); 2048 rows, 2 of 8, 4096 to 14336 892 us (bf16; 1.6 PFLOP/s).
 #include <algorithm>
 
 #include "experts.h"
@@ -788,8 +788,14 @@ hipError_t launch_experts(const ExpertSet &e, const ExpertCall &c, void *scratch
     if (c.bf16) hipLaunchKernelGGL((expert_rows<true>), rows, dim3(256), 0, s, x, xld, l.p, d, nkb, l.x);
     else hipLaunchKernelGGL((expert_rows<false>), rows, dim3(256), 0, s, x, xld, l.p, d, nkb, l.x);
     if ((err = hipGetLastError()) != hipSuccess) return err;
-    if ((err = launch_fp8_grouped(e.gate, &e.up, e.act, l.p, l.x, l.h, nullptr, s)) != hipSuccess) return err;
-    if ((err = launch_fp8_grouped(e.down, nullptr, 0, l.p, l.h, l.h, l.part, s)) != hipSuccess) return err;
+    // The 8-bit instructions' dropped bits (fp8_mfma) move a hidden value next to the border of
+    // two codes to the other one, 0.0011 of the result's 2-norm where f32 sums move 0.0002. An
+    // f16 result and f32 rows would show that; bf16's own rounding is 0.0017 (3001 rows, 8 of
+    // 128 experts, 2048 to 1000: 407 us with 8-bit products, 532 with f16 ones; 2048 rows, 2 of
+    // 8, 4096 to 14336: 892 and 1322).
+    const bool exact = c.y != nullptr || !c.bf16;
+    if ((err = launch_fp8_grouped(e.gate, &e.up, e.act, l.p, l.x, l.h, nullptr, exact, s)) != hipSuccess) return err;
+    if ((err = launch_fp8_grouped(e.down, nullptr, 0, l.p, l.h, l.h, l.part, false, s)) != hipSuccess) return err;
     return c.bf16 ? launch_sum<true>(c, l.part, l.p.place, experts, d, s) : launch_sum<false>(c, l.part, l.p.place, experts, d, s);
 }
 

@@ -90,12 +90,12 @@ __device__ __forceinline__ float4_t fp8_mfma(const int8x_t &w, const int8x_t &a,
                                                             (int)e);
 }
 
-// Eight codes (two dwords) as f16 values, exact.
+// Two codes (a dword's low or high half) as f16 values, exact; eight (two dwords).
+__device__ __forceinline__ half2_t fp8_pair_f16(uint32_t a, bool high) {
+    return high ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, 1.0f, true) : __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, 1.0f, false);
+}
 __device__ __forceinline__ half8_t fp8_to_f16(uint32_t a, uint32_t b) {
-    const half2_t x = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, 1.0f, false);
-    const half2_t y = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, 1.0f, true);
-    const half2_t z = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, 1.0f, false);
-    const half2_t w = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, 1.0f, true);
+    const half2_t x = fp8_pair_f16(a, false), y = fp8_pair_f16(a, true), z = fp8_pair_f16(b, false), w = fp8_pair_f16(b, true);
     return (half8_t){x[0], x[1], y[0], y[1], z[0], z[1], w[0], w[1]};
 }
 // The codes' sums of a fragment by f16 products, which drop nothing of them, at a quarter

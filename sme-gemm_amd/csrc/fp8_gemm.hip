@@ -12,6 +12,8 @@
 // expert's. GLU: a wave's column halves are 32 gate and the same 32 up columns, so that
 // a lane holds both factors of a hidden value; the tile's 128 hidden columns are one
 // block of the next product's depths, which the store quantizes into its fragments.
+// GLU16: tiles of 128 rows over v_mfma_f32_16x16x32_f16 of the codes, widened in registers,
+// for results that would show the 8-bit instructions' dropped bits (launch_experts).
 #include <algorithm>
 #include <type_traits>
 
@@ -40,7 +42,8 @@ struct F8Args {
     uint32_t hkb;               // blocks of the hidden width
 };
 
-enum F8Mode : int { F8_DENSE = 0, F8_GROUPED = 1, F8_GLU = 2 };
+enum F8Mode : int { F8_DENSE = 0, F8_GROUPED = 1, F8_GLU = 2, F8_GLU16 = 3 };
+constexpr bool f8_glu(int mode) { return mode >= F8_GLU; }
 
 // A weight block's scales for 64 consecutive blocks of K, one a lane, read back by
 // v_readlane: a scalar operand for the fold without a memory wait in the loop.
@@ -158,7 +161,7 @@ struct F8Place {
 };
 template <int BM, int BN, int MODE>
 __device__ __forceinline__ bool f8_place(const F8Args &f, DArgs &g, F8Place &p) {
-    constexpr int CN = MODE == F8_GLU ? BN / 2 : BN;  // columns a tile stands for
+    constexpr int CN = f8_glu(MODE) ? BN / 2 : BN;  // columns a tile stands for
     p.codes = f.w;
     p.codes2 = f.w2;
     p.scales = f.sw;
@@ -183,26 +186,29 @@ __device__ __forceinline__ bool f8_place(const F8Args &f, DArgs &g, F8Place &p) 
         }
     } else {
         const uint32_t count = f.head[EXPERT_TILES];
-        if (blockIdx.x >= count * nt) return false;  // (the grid is what any plan may need)
+        constexpr uint32_t SPLIT = 256 / BM;  // tiles of 128 rows: two of each of the plan's
+        if (blockIdx.x >= count * nt * SPLIT) return false;  // (the grid is what any plan may need)
         // An XCD's workgroups take a contiguous run of an expert's rows tiles x columns, rows
         // first, so that the expert's weights stay in its L2 from one row tile to the next
         // (bands of 2, 4, 8 and 16 row tiles of any expert took 326, 335, 341 and 341 us for
         // both products of 24008 rows over 128 experts and 896, 870, 900 and 880 for 4096
         // over 8; this 315 and 865).
-        const uint32_t l = xcd_tile(blockIdx.x, count * nt);
-        const ExpertTile s = f.tiles[l / nt];
-        const uint32_t first = __builtin_amdgcn_readfirstlane((int)s.first), own = __builtin_amdgcn_readfirstlane((int)s.count);
-        const uint32_t in = l - first * nt;
+        const uint32_t l = xcd_tile(blockIdx.x, count * nt * SPLIT);
+        const ExpertTile s = f.tiles[l / (nt * SPLIT)];
+        const uint32_t first = __builtin_amdgcn_readfirstlane((int)s.first);
+        const uint32_t own = __builtin_amdgcn_readfirstlane((int)s.count) * SPLIT;
+        const uint32_t in = l - first * nt * SPLIT;
         tm = in % own;
         p.tn = in / own;
-        p.rt0 = __builtin_amdgcn_readfirstlane((int)s.rt) + tm * 16;
+        p.rt0 = __builtin_amdgcn_readfirstlane((int)s.rt) + tm * (BM / 16);
         p.rt_end = __builtin_amdgcn_readfirstlane((int)s.rt_end);
         p.half = tm + 1 == own && __builtin_amdgcn_readfirstlane((int)s.half) != 0;
+        if (SPLIT > 1 && p.rt0 >= p.rt_end) return false;
         g.st.m = p.rt_end * 16;
         const size_t x = (uint32_t)__builtin_amdgcn_readfirstlane((int)s.expert);
         p.codes += x * f.n16 * f.nkb * FP8_FRAG;
         p.scales += x * (f.n16 / 8) * f.nkb;
-        if constexpr (MODE == F8_GLU) {
+        if constexpr (f8_glu(MODE)) {
             p.codes2 += x * f.n16 * f.nkb * FP8_FRAG;
             p.scales2 += x * (f.n16 / 8) * f.nkb;
         }
@@ -216,7 +222,7 @@ template <int BN, int NJ, int MODE>
 __device__ __forceinline__ const uint8_t *f8_columns(const F8Args &f, const F8Place &p, uint32_t c) {
     const uint8_t *base = p.codes;
     uint32_t tile;
-    if constexpr (MODE == F8_GLU) {
+    if constexpr (f8_glu(MODE)) {
         if (c % NJ >= NJ / 2) base = p.codes2;
         tile = p.tn * (BN / 32) + c / NJ * (NJ / 2) + c % (NJ / 2);
     } else {
@@ -227,7 +233,7 @@ __device__ __forceinline__ const uint8_t *f8_columns(const F8Args &f, const F8Pl
 // The block of 128 columns that wave column wc's slots lie in.
 template <int BN, int NJ, int MODE>
 __device__ __forceinline__ uint32_t f8_block(const F8Args &f, const F8Place &p, uint32_t wc) {
-    if constexpr (MODE == F8_GLU) return (p.tn * (BN / 32) + wc * (NJ / 2)) / 8;
+    if constexpr (f8_glu(MODE)) return (p.tn * (BN / 32) + wc * (NJ / 2)) / 8;
     else return min((p.tn * BN + wc * NJ * 16) / 128, f.n16 / 8 - 1);
 }
 
@@ -436,6 +442,8 @@ __device__ __forceinline__ void f8_big(const F8Args &f, const EpArgs &ep, const 
         dma_rows(step, 0);
     };
 
+    constexpr bool EXACT = MODE == F8_GLU16;
+    static_assert(!EXACT || PH == 1, "the f16 fragments' registers");
     float4_t acc[PH * RT][4], part[4];
 #pragma unroll
     for (int i = 0; i < PH * RT; i++)
@@ -446,14 +454,14 @@ __device__ __forceinline__ void f8_big(const F8Args &f, const EpArgs &ep, const 
     int8x_t a[RT], w[4];
     uint32_t e = 0;
     const float *scales = pl.scales + (size_t)f8_block<BN, 4, MODE>(f, pl, wc) * f.nkb;
-    const float *scales2 = MODE == F8_GLU ? pl.scales2 + (size_t)f8_block<BN, 4, MODE>(f, pl, wc) * f.nkb : nullptr;
+    const float *scales2 = f8_glu(MODE) ? pl.scales2 + (size_t)f8_block<BN, 4, MODE>(f, pl, wc) * f.nkb : nullptr;
     float sl = 0.0f, sl2 = 0.0f, sw = 0.0f, sw2 = 0.0f;
     const uint32_t fa = lds0 + T::W + wr * RT * FP8_FRAG + lane * 16, fw = lds0 + wc * 4 * FP8_FRAG + lane * 16;
 
     // product p of a phase: row tile p / 4, column tile p % 4; folded LAG products later
     constexpr int N = 4 * RT, LAG = 3;
     auto fold = [&](int h, int p) __attribute__((always_inline)) {
-        fp8_fold(acc[h * RT + p / 4][p % 4], part[p % 4], MODE == F8_GLU && p % 4 >= 2 ? sw2 : sw);
+        fp8_fold(acc[h * RT + p / 4][p % 4], part[p % 4], f8_glu(MODE) && p % 4 >= 2 ? sw2 : sw);
     };
     auto read_rows = [&](uint32_t step, int h) __attribute__((always_inline)) {
         const uint32_t st = step % T::NS;
@@ -495,9 +503,59 @@ __device__ __forceinline__ void f8_big(const F8Args &f, const EpArgs &ep, const 
         barrier_lds();
         __builtin_amdgcn_sched_barrier(0);
     };
-    auto rest = [&](int h) __attribute__((always_inline)) {
+    // F8_GLU16: the same products of the codes' f16 values, which drop nothing: four
+    // instructions for a block's depths, four column tiles side by side, each followed by its
+    // share of the next row tile's widening and of the last one's folds, which issue while the
+    // matrix core works.
+    half8_t a16[2][4], w16[EXACT ? 4 : 1][4];
+    float4_t p16[2][4];
+    float s16[2][2];  // the row's scale times the gate's and the up weights', by p16's row tile
+    if constexpr (EXACT) {
 #pragma unroll
-        for (int p = N - LAG; p < N; p++) fold(h, p);
+        for (int j = 0; j < 4; j++) p16[(RT - 1) & 1][j] = (float4_t){0.f, 0.f, 0.f, 0.f};
+        s16[(RT - 1) & 1][0] = s16[(RT - 1) & 1][1] = 0.0f;
+    }
+    auto fold16 = [&](int i, int j, int v) __attribute__((always_inline)) {
+        acc[i][j][v] = __builtin_fmaf(p16[i & 1][j][v], s16[i & 1][j / 2], acc[i][j][v]);
+    };
+    auto mul_exact = [&]() __attribute__((always_inline)) {
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int i = 0; i < RT; i++) {
+#pragma unroll
+            for (int c = 0; c < 4; c++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const float4_t z = {0.f, 0.f, 0.f, 0.f};
+                    if (i == 0) {
+                        if (j == 0) a16[0][c] = fp8_to_f16(a[0][2 * c], a[0][2 * c + 1]);
+                        w16[j][c] = fp8_to_f16(w[j][2 * c], w[j][2 * c + 1]);
+                    }
+                    p16[i & 1][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w16[j][c], a16[i & 1][c], c == 0 ? z : p16[i & 1][j], 0, 0, 0);
+                    if (i + 1 < RT) {
+                        const half2_t x = fp8_pair_f16(a[i + 1][2 * c + j / 2], j % 2);
+                        a16[(i + 1) & 1][c][2 * j] = x[0];
+                        a16[(i + 1) & 1][c][2 * j + 1] = x[1];
+                    }
+                    if (i > 0) fold16(i - 1, c, j);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            const float rs = __uint_as_float((e >> (8 * i) & 0xFF) << 23);
+            s16[i & 1][0] = sw * rs;
+            s16[i & 1][1] = sw2 * rs;
+        }
+        __builtin_amdgcn_s_setprio(0);
+        barrier_lds();
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    auto rest = [&](int h) __attribute__((always_inline)) {
+        if constexpr (EXACT) {
+#pragma unroll
+            for (int p = 0; p < 16; p++) fold16(RT - 1, p / 4, p % 4);
+        } else {
+#pragma unroll
+            for (int p = N - LAG; p < N; p++) fold(h, p);
+        }
     };
     constexpr std::integral_constant<int, 0> h0;
     constexpr std::integral_constant<int, PH - 1> h1;
@@ -517,12 +575,13 @@ __device__ __forceinline__ void f8_big(const F8Args &f, const EpArgs &ep, const 
             rest(PH - 1);  // (the step before's)
             if (ks % 64 == 0) {
                 sl = scale_lane(scales, ks, f.nkb, lane);
-                if constexpr (MODE == F8_GLU) sl2 = scale_lane(scales2, ks, f.nkb, lane);
+                if constexpr (f8_glu(MODE)) sl2 = scale_lane(scales2, ks, f.nkb, lane);
             }
             sw = scale_at(sl, ks);
-            if constexpr (MODE == F8_GLU) sw2 = scale_at(sl2, ks);
+            if constexpr (f8_glu(MODE)) sw2 = scale_at(sl2, ks);
             mem_end();
-            mul(h0);
+            if constexpr (EXACT) mul_exact();
+            else mul(h0);
             if constexpr (PH == 2) {
                 read_rows(ks, 1);
                 dma_first(ks + 2);
@@ -542,7 +601,7 @@ __device__ __forceinline__ void f8_big(const F8Args &f, const EpArgs &ep, const 
     int to = t;
     asm volatile("" : "+v"(to));
     const int lro = to % 16, lgo = to % 64 / 16;
-    if constexpr (MODE == F8_GLU) {
+    if constexpr (f8_glu(MODE)) {
         glu_store<PH * RT, 4>(f, acc, (uint32_t *)ring, rt0, pl.rt_end, tn, wr, wc, to % 64);
         return;
     }
@@ -602,9 +661,13 @@ __global__ void __launch_bounds__(512, 2) fp8_big(F8Args f, EpArgs ep) {
     __shared__ __align__(1024) uint8_t ring[F8Big<256>::LDS > F8Big<128>::LDS ? F8Big<256>::LDS : F8Big<128>::LDS];
     DArgs g = f.d;
     F8Place pl;
-    if (!f8_place<256, 256, MODE>(f, g, pl)) return;
-    if (pl.half) f8_big<128, BF16, EPV, MODE>(f, ep, g, pl, ring);
-    else f8_big<256, BF16, EPV, MODE>(f, ep, g, pl, ring);
+    if (!f8_place<MODE == F8_GLU16 ? 128 : 256, 256, MODE>(f, g, pl)) return;
+    if constexpr (MODE == F8_GLU16) {
+        f8_big<128, BF16, EPV, MODE>(f, ep, g, pl, ring);
+    } else {
+        if (pl.half) f8_big<128, BF16, EPV, MODE>(f, ep, g, pl, ring);
+        else f8_big<256, BF16, EPV, MODE>(f, ep, g, pl, ring);
+    }
 }
 
 // Where the last round of 256-row tiles would leave half of the compute units or more
@@ -721,7 +784,7 @@ hipError_t launch_fp8_gemm(const Fp8Mat &w, size_t m, uint16_t *dst, Fp8Rows a, 
 }
 
 hipError_t launch_fp8_grouped(const Fp8Mat &w, const Fp8Mat *up, uint32_t act, const ExpertPlan &p, Fp8Rows a, Fp8Rows h,
-                              float *dst, hipStream_t s) {
+                              float *dst, bool exact, hipStream_t s) {
     F8Args f = {};
     DArgs &g = f.d;
     g.st.dst = (uint16_t *)dst;
@@ -736,7 +799,7 @@ hipError_t launch_fp8_grouped(const Fp8Mat &w, const Fp8Mat *up, uint32_t act, c
     f.head = p.head;
     f.tiles = p.tiles;
     const uint32_t cols = up ? 128 : 256;
-    const dim3 grid(p.max_tiles * ((w.n + cols - 1) / cols)), block(512);
+    const dim3 grid(p.max_tiles * (up && exact ? 2 : 1) * ((w.n + cols - 1) / cols)), block(512);
     if (grid.x == 0) return hipSuccess;
     if (up) {
         f.w2 = up->codes;
@@ -746,7 +809,8 @@ hipError_t launch_fp8_grouped(const Fp8Mat &w, const Fp8Mat *up, uint32_t act, c
         f.he = h.e;
         f.hkb = w.n16 / 8;
     }
-    if (up) hipLaunchKernelGGL((fp8_big<false, 1, F8_GLU>), grid, block, 0, s, f, EpArgs{});
+    if (up && exact) hipLaunchKernelGGL((fp8_big<false, 1, F8_GLU16>), grid, block, 0, s, f, EpArgs{});
+    else if (up) hipLaunchKernelGGL((fp8_big<false, 1, F8_GLU>), grid, block, 0, s, f, EpArgs{});
     else hipLaunchKernelGGL((fp8_big<false, 1, F8_GROUPED>), grid, block, 0, s, f, EpArgs{});
     return hipGetLastError();
 }

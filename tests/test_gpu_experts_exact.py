@@ -152,3 +152,37 @@ def test_experts_past_4_gb(smg, rows):
     xv = exact.rows_of(rng, rows, d)
     want, off, _ = exact.experts(xv, parts, few, w)
     check(values(run_experts(e, bits(xv, True), ids, w, True), True), want, off, True, f"{rows} rows")
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("rows", [1, 40, 300])
+def test_hidden_values_keep_their_codes(smg, rows, bf16):
+    """Random weights: the error of the whole by its 2-norm. f32 sums of a few thousand
+    products are off by less than 2^-21 of their 2-norm, and the hidden values by twice that;
+    codes lie 2^-4 of a value apart or more, so one in 2^-20 2^5 takes its neighbour, a step of
+    2^-3 of it at most: sqrt(2^-15) 2^-3 = 2^-10.5 of the whole. The second product's dropped
+    bits (2^-16) and an f16 result's rounding (2^-11 / sqrt(3)) add up to less than 2^-11.5.
+    In f32 rows the same without the rounding; bf16 results are not held to it."""
+    rng = np.random.default_rng(rows)
+    experts, d, ffn, k = 4, 2048, 768, 2
+    parts = []
+    for n, kk in ((ffn, d), (ffn, d), (d, ffn)):
+        v = ref.e4m3_round(np.clip(rng.standard_normal((experts, n, kk)) * 112, -448, 448))
+        s = (rng.uniform(0.7, 1.3, (experts, -(-n // 128), -(-kk // 128))) / (112 * np.sqrt(kk))).astype(np.float32)
+        c = exact.code_of(v)
+        parts.append((c, s, np.stack([ref.weights(ci, si, n, kk) for ci, si in zip(c, s)])))
+    e = build(smg, parts, experts, d, ffn)
+    x = bits(rng.standard_normal((rows, d)), bf16)
+    ids = np.stack([rng.permutation(experts)[:k] for _ in range(rows)]).astype(np.int32)
+    w = rng.uniform(0.1, 1, (rows, k)).astype(np.float32)
+    a, want = ref.quantize_rows(values(x, bf16)), np.zeros((rows, d))
+    for i in range(experts):
+        r, j = np.nonzero(ids == i)
+        h = ref.act(a[r] @ parts[0][2][i].T, False) * (a[r] @ parts[1][2][i].T)
+        np.add.at(want, r, w[r, j][:, None].astype(np.float64) * (ref.quantize_rows(h) @ parts[2][2][i].T))
+    got = [accumulate(e, x, ids, w, np.zeros((rows, d), np.float32), bf16)]
+    if not bf16:
+        got.append(values(run_experts(e, x, ids, w, False), False))
+    for g in got:
+        err = np.linalg.norm(g - want) / np.linalg.norm(want)
+        assert err < 2.0 ** -10, err
