@@ -12,6 +12,7 @@
 #include <map>
 #include <memory>
 #include <mutex>
+#include <string>
 #include <utility>
 
 #include "api_internal.h"
@@ -43,14 +44,12 @@ class CallScratch {
 public:
     // `bytes` (0: none) for a call on (device, stream), the device being current.
     CallScratch(int device, void *stream, size_t bytes) {
-        if (bytes == 0) {
-            ok_ = true;
-            return;
-        }
+        if (bytes == 0) return;
         hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
         unsigned long long id = 0;
-        if (hipStreamGetCaptureInfo((hipStream_t)stream, &st, &id) != hipSuccess) {
-            (void)hipGetLastError();  // (the null stream beside another one's capture: the launches report it)
+        error_ = hipStreamGetCaptureInfo((hipStream_t)stream, &st, &id);
+        if (error_ != hipSuccess) {  // (the null stream beside a blocking one's capture)
+            (void)hipGetLastError();
             return;
         }
         // each thread's own stream has one handle
@@ -68,16 +67,24 @@ public:
             std::unique_ptr<char> &k = (*keys)[{id, key}];
             if (!k) k.reset(new char);
             buf_ = pool->get(device, k.get(), bytes);
+        } else {
+            error_ = hipErrorStreamCaptureInvalidated;
+            return;
         }
-        ok_ = buf_ != nullptr;
+        if (!buf_) error_ = hipErrorOutOfMemory;
     }
-    bool ok() const { return ok_; }
+    // SMG_OK, or the failure, reported for `call`.
+    int check(const char *call) const {
+        if (error_ == hipSuccess) return SMG_OK;
+        if (error_ == hipErrorOutOfMemory) return report(SMG_ENOMEM, (std::string(call) + ": scratch hipMalloc").c_str());
+        return report_hip(SMG_EHIP, call, error_);
+    }
     void *buf() const { return buf_; }
 
 private:
     LeasePool<CallAlloc>::Lease lease_;
     void *buf_ = nullptr;
-    bool ok_ = false;
+    hipError_t error_ = hipSuccess;
 };
 
 // Makes a device current for a scope.

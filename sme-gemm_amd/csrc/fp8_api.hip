@@ -187,7 +187,7 @@ int experts_dev(const smg_experts *e, const uint16_t *x, int bf16, const int32_t
     const ExpertSet set = e->set();
     const ExpertCall c = {x, ids, weights, out, y, (uint32_t)rows, (uint32_t)top_k, bf16 != 0};
     CallScratch sc(e->device, stream, experts_scratch_bytes(set, c));
-    if (!sc.ok()) return report(SMG_ENOMEM, "experts: scratch hipMalloc");
+    if ((rc = sc.check("experts"))) return rc;
     const hipError_t err = launch_experts(set, c, sc.buf(), (hipStream_t)stream);
     return err == hipSuccess ? SMG_OK : report_hip(SMG_EHIP, "experts", err);
 }
@@ -359,7 +359,7 @@ int smg_fp8_matmul_dev(size_t m, const smg_weights *w, uint16_t *dst, const uint
         DeviceScope on(w->device);
         if (on.error() != hipSuccess) return report_hip(SMG_EHIP, "hipSetDevice", on.error());
         CallScratch sc(w->device, stream, fp8_scratch_bytes(w->f8, m));
-        if (!sc.ok()) return report(SMG_ENOMEM, "smg_fp8_matmul_dev: scratch hipMalloc");
+        if ((rc = sc.check("smg_fp8_matmul_dev"))) return rc;
         hipStream_t s = (hipStream_t)stream;
         hipError_t e = launch_fp8_matmul(w->f8, m, dst, lhs, p.fused, bf16 != 0, sc.buf(), s);
         if (e == hipSuccess) e = run_graph_tail(p, dst, m, n, bf16 != 0, s);
