@@ -336,10 +336,16 @@ int smg_q4_chained_dev(size_t m, const smg_weights *w, uint16_t *dst, const uint
  * kernel; others first, into scratch the call holds for its launches (calls of several
  * host threads on one stream stay apart). While the stream is captured the scratch is
  * the capture's own, allocated by the call and kept until the process ends: graphs
- * share none, with each other or with eager calls. dst overlaps neither lhs nor an
- * operand of another cell. */
+ * share none, with each other or with eager calls. A program that captures again and
+ * again uses the _ws form. dst overlaps neither lhs nor an operand of another cell. */
 int smg_fp8_matmul_dev(size_t m, const smg_weights *w, uint16_t *dst, const uint16_t *lhs, const ep_desc16 *ep,
                        int bf16, void *stream);
+/* smg_fp8_matmul_dev in the caller's scratch: `bytes` of device memory at a multiple of
+ * 256, at least smg_fp8_scratch_bytes' (which may be 0, scratch NULL), that nothing else
+ * uses until the call's work has run, or as long as a graph holds it. */
+int smg_fp8_scratch_bytes(const smg_weights *w, size_t m, size_t *bytes);
+int smg_fp8_matmul_ws_dev(size_t m, const smg_weights *w, uint16_t *dst, const uint16_t *lhs, const ep_desc16 *ep,
+                          int bf16, void *scratch, size_t bytes, void *stream);
 int smg_lowbit_matmul_dev(size_t m, const smg_weights *w, uint16_t *dst, const uint16_t *lhs,
                           const ep_desc16 *ep, void *stream);
 /* smg_lowbit_matmul_dev that allocates nothing. It has no counterpart in the
@@ -549,6 +555,14 @@ int smg_experts_forward_dev(const smg_experts *e, const uint16_t *x, int bf16, c
                             const float *weights, size_t rows, size_t top_k, uint16_t *out, void *stream);
 int smg_experts_accumulate_dev(const smg_experts *e, const uint16_t *x, int bf16, const int32_t *ids,
                                const float *weights, size_t rows, size_t top_k, float *y, void *stream);
+/* The same in the caller's scratch, as smg_fp8_matmul_ws_dev. */
+int smg_experts_scratch_bytes(const smg_experts *e, size_t rows, size_t top_k, size_t *bytes);
+int smg_experts_forward_ws_dev(const smg_experts *e, const uint16_t *x, int bf16, const int32_t *ids,
+                               const float *weights, size_t rows, size_t top_k, uint16_t *out, void *scratch,
+                               size_t bytes, void *stream);
+int smg_experts_accumulate_ws_dev(const smg_experts *e, const uint16_t *x, int bf16, const int32_t *ids,
+                                  const float *weights, size_t rows, size_t top_k, float *y, void *scratch,
+                                  size_t bytes, void *stream);
 
 /* ---- host-slice forms of the model parts ------------------------------------
  * The reference's model parts take host slices (&[X] / &mut [f32]). Each entry

@@ -6,7 +6,9 @@
 // until the process ends, as the graph may be launched at any time: no two graphs,
 // and no graph and eager call, share one. Within a capture the calls of one stream
 // are ordered by that stream and share a buffer; a branch captured from another
-// stream has its own.
+// stream has its own. A caller that brings scratch of its own uses that, and says when it
+// ends: HIP tells the library nothing when a graph does (a user object that the captured
+// graph retains is not released with the instantiated one).
 #pragma once
 
 #include <map>
@@ -40,10 +42,22 @@ struct CallAlloc {
     }
 };
 
+// A caller's scratch: on the call's device, at a multiple of 256 bytes.
+struct OwnScratch {
+    void *buf;
+    size_t bytes;
+};
+
 class CallScratch {
 public:
-    // `bytes` (0: none) for a call on (device, stream), the device being current.
-    CallScratch(int device, void *stream, size_t bytes) {
+    // `bytes` (0: none) for a call on (device, stream), the device being current; the
+    // caller's own, if there is one.
+    CallScratch(int device, void *stream, size_t bytes, const OwnScratch *mine) {
+        if (mine) {
+            buf_ = mine->buf;
+            if (bytes > mine->bytes || (bytes && (!buf_ || (uintptr_t)buf_ % 256))) error_ = hipErrorInvalidValue;
+            return;
+        }
         if (bytes == 0) return;
         hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
         unsigned long long id = 0;
@@ -76,6 +90,8 @@ public:
     // SMG_OK, or the failure, reported for `call`.
     int check(const char *call) const {
         if (error_ == hipSuccess) return SMG_OK;
+        if (error_ == hipErrorInvalidValue)
+            return report(SMG_EINVAL, (std::string(call) + ": scratch too small, or not at a multiple of 256 bytes").c_str());
         if (error_ == hipErrorOutOfMemory) return report(SMG_ENOMEM, (std::string(call) + ": scratch hipMalloc").c_str());
         return report_hip(SMG_EHIP, call, error_);
     }

@@ -66,6 +66,7 @@ struct ExpertCall {
     bool bf16;
 };
 size_t experts_scratch_bytes(const ExpertSet &e, const ExpertCall &c);
+size_t experts_scratch_bytes(const ExpertSet &e, size_t rows, size_t top_k);  // the most, x at any address
 hipError_t launch_experts(const ExpertSet &e, const ExpertCall &c, void *scratch, hipStream_t s);
 
 }  // namespace smg

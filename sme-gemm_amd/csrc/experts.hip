@@ -670,9 +670,9 @@ bool few_rows(size_t rows, size_t top_k, size_t experts) {
 
 // Whether the call's rows are copied to where they can be read 8 values at a time (one
 // row's kernels read two).
+bool may_pad(const ExpertSet &e, size_t rows, size_t top_k) { return !(rows == 1 && few_rows(rows, top_k, e.gate.mats)); }
 bool pads(const ExpertSet &e, const ExpertCall &c) {
-    return (e.gate.k % 8 != 0 || ((uintptr_t)c.x & 15) != 0) &&
-           !(c.rows == 1 && few_rows(c.rows, c.top_k, e.gate.mats));
+    return (e.gate.k % 8 != 0 || ((uintptr_t)c.x & 15) != 0) && may_pad(e, c.rows, c.top_k);
 }
 
 size_t up256(size_t x) { return (x + 255) / 256 * 256; }
@@ -728,6 +728,9 @@ Layout layout(const ExpertSet &e, size_t rows, size_t top_k, bool pads, void *sc
 
 size_t experts_scratch_bytes(const ExpertSet &e, const ExpertCall &c) {
     return layout(e, c.rows, c.top_k, pads(e, c), nullptr).bytes;
+}
+size_t experts_scratch_bytes(const ExpertSet &e, size_t rows, size_t top_k) {
+    return layout(e, rows, top_k, may_pad(e, rows, top_k), nullptr).bytes;
 }
 
 hipError_t launch_experts(const ExpertSet &e, const ExpertCall &c, void *scratch, hipStream_t s) {

@@ -160,11 +160,9 @@ int experts_create(const ExpertArrays &a, size_t experts, size_t d, size_t ffn, 
     return SMG_OK;
 }
 
-int experts_check(const smg_experts *e, const void *x, const int32_t *ids, const float *weights, const void *out, size_t rows,
-                  size_t top_k) {
+int experts_limits(const smg_experts *e, size_t rows, size_t top_k) {
     if (!e) return report(SMG_EINVAL, "null experts");
     if (top_k == 0) return report(SMG_EINVAL, "a row has at least one expert");
-    if (!x || !ids || !weights || !out) return report(SMG_EINVAL, "null array");
     const size_t big = (size_t)1 << 31;
     // (the kernels' grids: a wave per 16 padded rows and block of depths, a workgroup
     // per tile of 128 rows x 128 columns, one per 2048 columns of a row)
@@ -176,17 +174,24 @@ int experts_check(const smg_experts *e, const void *x, const int32_t *ids, const
     return SMG_OK;
 }
 
+int experts_check(const smg_experts *e, const void *x, const int32_t *ids, const float *weights, const void *out, size_t rows,
+                  size_t top_k) {
+    const int rc = experts_limits(e, rows, top_k);
+    if (rc) return rc;
+    return x && ids && weights && out ? SMG_OK : report(SMG_EINVAL, "null array");
+}
+
 int experts_dev(const smg_experts *e, const uint16_t *x, int bf16, const int32_t *ids, const float *weights, size_t rows,
-                size_t top_k, uint16_t *out, float *y, void *stream) {
+                size_t top_k, uint16_t *out, float *y, void *stream, const OwnScratch *own = nullptr) {
     if (e && rows == 0) return SMG_OK;
     int rc = experts_check(e, x, ids, weights, out ? (const void *)out : y, rows, top_k);
     if (rc) return rc;
-    if ((rc = check_device_pointers(e->device, EpPlan{}, {x, ids, weights, out, y}))) return rc;
+    if ((rc = check_device_pointers(e->device, EpPlan{}, {x, ids, weights, out, y, own ? own->buf : nullptr}))) return rc;
     DeviceScope on(e->device);
     if (on.error() != hipSuccess) return report_hip(SMG_EHIP, "hipSetDevice", on.error());
     const ExpertSet set = e->set();
     const ExpertCall c = {x, ids, weights, out, y, (uint32_t)rows, (uint32_t)top_k, bf16 != 0};
-    CallScratch sc(e->device, stream, experts_scratch_bytes(set, c));
+    CallScratch sc(e->device, stream, experts_scratch_bytes(set, c), own);
     if ((rc = sc.check("experts"))) return rc;
     const hipError_t err = launch_experts(set, c, sc.buf(), (hipStream_t)stream);
     return err == hipSuccess ? SMG_OK : report_hip(SMG_EHIP, "experts", err);
@@ -208,6 +213,27 @@ int experts_host(const smg_experts *e, const uint16_t *x, int bf16, const int32_
         return experts_dev(e, (const uint16_t *)d[0], bf16, (const int32_t *)d[1], (const float *)d[2], rows, top_k,
                            (uint16_t *)d[3], (float *)d[4], st);
     });
+}
+
+int fp8_dev(size_t m, const smg_weights *w, uint16_t *dst, const uint16_t *lhs, const ep_desc16 *ep, int bf16, void *stream,
+            const OwnScratch *own) {
+    int rc = check_fp8(w);
+    if (rc) return rc;
+    const size_t n = w->d.n, k = w->d.k;
+    if (m == 0 || n == 0) return SMG_OK;
+    if (!dst || (k && !lhs)) return report(SMG_EINVAL, "null array");
+    if ((rc = check_rows(w, m))) return rc;
+    EpPlan p;
+    if ((rc = plan_graph(ep, &p, n))) return rc;
+    if ((rc = check_device_pointers(w->device, p, {dst, k ? lhs : nullptr, own ? own->buf : nullptr}))) return rc;
+    DeviceScope on(w->device);
+    if (on.error() != hipSuccess) return report_hip(SMG_EHIP, "hipSetDevice", on.error());
+    CallScratch sc(w->device, stream, fp8_scratch_bytes(w->f8, m), own);
+    if ((rc = sc.check("smg_fp8_matmul_dev"))) return rc;
+    hipStream_t s = (hipStream_t)stream;
+    hipError_t e = launch_fp8_matmul(w->f8, m, dst, lhs, p.fused, bf16 != 0, sc.buf(), s);
+    if (e == hipSuccess) e = run_graph_tail(p, dst, m, n, bf16 != 0, s);
+    return e == hipSuccess ? SMG_OK : report_hip(SMG_EHIP, "smg_fp8_matmul_dev", e);
 }
 
 int route_check(const smg_router *r, size_t rows, const void *logits, int type, const int32_t *ids, const float *weights) {
@@ -291,6 +317,26 @@ int smg_experts_accumulate_dev(const smg_experts *e, const uint16_t *x, int bf16
     return guarded([&] { return experts_dev(e, x, bf16, ids, weights, rows, top_k, nullptr, y, stream); });
 }
 
+int smg_experts_scratch_bytes(const smg_experts *e, size_t rows, size_t top_k, size_t *bytes) {
+    if (!bytes) return report(SMG_EINVAL, "null argument");
+    const int rc = experts_limits(e, rows, top_k);
+    if (rc) return rc;
+    *bytes = rows ? experts_scratch_bytes(e->set(), rows, top_k) : 0;
+    return SMG_OK;
+}
+
+int smg_experts_forward_ws_dev(const smg_experts *e, const uint16_t *x, int bf16, const int32_t *ids, const float *weights,
+                               size_t rows, size_t top_k, uint16_t *out, void *scratch, size_t bytes, void *stream) {
+    const OwnScratch own = {scratch, bytes};
+    return guarded([&] { return experts_dev(e, x, bf16, ids, weights, rows, top_k, out, nullptr, stream, &own); });
+}
+
+int smg_experts_accumulate_ws_dev(const smg_experts *e, const uint16_t *x, int bf16, const int32_t *ids, const float *weights,
+                                  size_t rows, size_t top_k, float *y, void *scratch, size_t bytes, void *stream) {
+    const OwnScratch own = {scratch, bytes};
+    return guarded([&] { return experts_dev(e, x, bf16, ids, weights, rows, top_k, nullptr, y, stream, &own); });
+}
+
 int smg_experts_forward(const smg_experts *e, const uint16_t *x, int bf16, const int32_t *ids, const float *weights, size_t rows,
                         size_t top_k, uint16_t *out) {
     return guarded([&] { return experts_host(e, x, bf16, ids, weights, rows, top_k, out, nullptr); });
@@ -346,25 +392,22 @@ int gemm_gpu_b16_fp8(size_t m, const smg_weights *w, uint16_t *dst, const uint16
 
 int smg_fp8_matmul_dev(size_t m, const smg_weights *w, uint16_t *dst, const uint16_t *lhs, const ep_desc16 *ep, int bf16,
                        void *stream) {
-    return guarded([&]() -> int {
-        int rc = check_fp8(w);
-        if (rc) return rc;
-        const size_t n = w->d.n, k = w->d.k;
-        if (m == 0 || n == 0) return SMG_OK;
-        if (!dst || (k && !lhs)) return report(SMG_EINVAL, "null array");
-        if ((rc = check_rows(w, m))) return rc;
-        EpPlan p;
-        if ((rc = plan_graph(ep, &p, n))) return rc;
-        if ((rc = check_device_pointers(w->device, p, {dst, k ? lhs : nullptr}))) return rc;
-        DeviceScope on(w->device);
-        if (on.error() != hipSuccess) return report_hip(SMG_EHIP, "hipSetDevice", on.error());
-        CallScratch sc(w->device, stream, fp8_scratch_bytes(w->f8, m));
-        if ((rc = sc.check("smg_fp8_matmul_dev"))) return rc;
-        hipStream_t s = (hipStream_t)stream;
-        hipError_t e = launch_fp8_matmul(w->f8, m, dst, lhs, p.fused, bf16 != 0, sc.buf(), s);
-        if (e == hipSuccess) e = run_graph_tail(p, dst, m, n, bf16 != 0, s);
-        return e == hipSuccess ? SMG_OK : report_hip(SMG_EHIP, "smg_fp8_matmul_dev", e);
-    });
+    return guarded([&] { return fp8_dev(m, w, dst, lhs, ep, bf16, stream, nullptr); });
+}
+
+int smg_fp8_scratch_bytes(const smg_weights *w, size_t m, size_t *bytes) {
+    int rc = check_fp8(w);
+    if (rc) return rc;
+    if (!bytes) return report(SMG_EINVAL, "null argument");
+    if ((rc = check_rows(w, m))) return rc;
+    *bytes = m && w->d.n ? fp8_scratch_bytes(w->f8, m) : 0;
+    return SMG_OK;
+}
+
+int smg_fp8_matmul_ws_dev(size_t m, const smg_weights *w, uint16_t *dst, const uint16_t *lhs, const ep_desc16 *ep, int bf16,
+                          void *scratch, size_t bytes, void *stream) {
+    const OwnScratch own = {scratch, bytes};
+    return guarded([&] { return fp8_dev(m, w, dst, lhs, ep, bf16, stream, &own); });
 }
 
 }  // extern "C"

@@ -76,6 +76,8 @@ def lib() -> C.CDLL:
     L.smg_fp8_create_dev.argtypes = [P, P, SZ, SZ, P, W]
     L.smg_fp8_quantize.argtypes = [P, C.c_int, SZ, SZ, P, P]
     L.smg_fp8_matmul_dev.argtypes = [SZ, P, P, P, P, C.c_int, P]
+    L.smg_fp8_scratch_bytes.argtypes = [P, SZ, C.POINTER(SZ)]
+    L.smg_fp8_matmul_ws_dev.argtypes = [SZ, P, P, P, P, C.c_int, P, SZ, P]
     L.smg_f16_prepack.argtypes = [P, SZ, SZ, C.c_long, C.c_long, W]
     L.smg_bf16_prepack.argtypes = [P, SZ, SZ, C.c_long, C.c_long, W]
     L.smg_q4_dequant.argtypes = [P, C.c_int, W]
@@ -116,6 +118,9 @@ def lib() -> C.CDLL:
     L.smg_experts_destroy.restype = None
     L.smg_experts_forward_dev.argtypes = [P, P, C.c_int, P, P, SZ, SZ, P, P]
     L.smg_experts_accumulate_dev.argtypes = [P, P, C.c_int, P, P, SZ, SZ, P, P]
+    L.smg_experts_scratch_bytes.argtypes = [P, SZ, SZ, C.POINTER(SZ)]
+    L.smg_experts_forward_ws_dev.argtypes = [P, P, C.c_int, P, P, SZ, SZ, P, P, SZ, P]
+    L.smg_experts_accumulate_ws_dev.argtypes = [P, P, C.c_int, P, P, SZ, SZ, P, P, SZ, P]
     L.smg_experts_forward.argtypes = [P, P, C.c_int, P, P, SZ, SZ, P]
     L.smg_experts_accumulate.argtypes = [P, P, C.c_int, P, P, SZ, SZ, P]
     # the decode block
@@ -895,6 +900,12 @@ class Fp8Weights(_Handle):
             _check(lib().smg_fp8_create(_ptr(codes), _ptr(scales), n, k, C.byref(h)), "smg_fp8_create")
         super().__init__(h, n, k)
 
+    def scratch_bytes(self, m: int) -> int:
+        """The scratch of a product of m rows (0: none)."""
+        b = SZ()
+        _check(lib().smg_fp8_scratch_bytes(self._h, m, C.byref(b)), "smg_fp8_scratch_bytes")
+        return b.value
+
     @classmethod
     def quantize(cls, w, layout: int, n: int, k: int) -> "Fp8Weights":
         """f32 weights in `layout` (WeightLayout.OutIn / InOut): quantize_fp8_arrays,
@@ -1012,7 +1023,18 @@ def _is_devn(x, n: int, device: int, dtype) -> bool:
     return x.dtype is dtype and x.get_device() == device and x.numel() == n and x.is_contiguous()
 
 
-def _matmul_fp8(a, w: Fp8Weights, c, m: int, ep, bf16: bool):
+def _own_scratch(x, device: int):
+    """(address, bytes) of a caller's scratch: a contiguous device tensor."""
+    if not _is_dev(x):
+        raise TypeError("scratch is a device tensor")
+    if not x.is_contiguous():
+        raise ValueError("scratch must be contiguous")
+    if x.get_device() != device:
+        raise ValueError(f"scratch is on cuda:{x.get_device()}, expected cuda:{device}")
+    return x.data_ptr(), x.numel() * x.element_size()
+
+
+def _matmul_fp8(a, w: Fp8Weights, c, m: int, ep, bf16: bool, scratch=None):
     n, k = w._n, w._k
     plain = ep is None or not ep.nodes and ep.act is None
     if not plain and ep.bf16 != bf16:
@@ -1020,6 +1042,8 @@ def _matmul_fp8(a, w: Fp8Weights, c, m: int, ep, bf16: bool):
     dev, t = w._on, _torch16(bf16)
     if not (_is_dev(a) and _is_dev(c) and _is_devn(a, m * k, dev, t) and _is_devn(c, m * n, dev, t)):
         if not _same_side(a, c):
+            if scratch is not None:
+                raise TypeError("scratch belongs to calls of device tensors")
             return _run_host_or_dev("gemm_gpu_b16_fp8" if bf16 else "gemm_gpu_f16_fp8", None, a, w, c, m, ep)
         _dev16(a, m * k, "a (m*k)", dev, bf16)
         _dev16(c, m * n, "c (m*n)", dev, bf16)
@@ -1028,30 +1052,36 @@ def _matmul_fp8(a, w: Fp8Weights, c, m: int, ep, bf16: bool):
     else:
         ep.validate(m, n, dev)
         eptr, keep = ep.packed(n)
-    rc = _lib.smg_fp8_matmul_dev(m, w._h, c.data_ptr(), a.data_ptr(), eptr, bf16, _stream_on(dev))
+    if scratch is None:
+        rc = _lib.smg_fp8_matmul_dev(m, w._h, c.data_ptr(), a.data_ptr(), eptr, bf16, _stream_on(dev))
+    else:
+        rc = _lib.smg_fp8_matmul_ws_dev(m, w._h, c.data_ptr(), a.data_ptr(), eptr, bf16, *_own_scratch(scratch, dev),
+                                        _stream_on(dev))
     if rc:
         _check(rc, "smg_fp8_matmul_dev")
     return c
 
 
-def matmul_fp8_ep(a, w: Fp8Weights, c, m: int, ep: Epilogue):
+def matmul_fp8_ep(a, w: Fp8Weights, c, m: int, ep: Epilogue, scratch=None):
     """c = ep(a @ w) for f16 a (m x k): each row's block of 128 depths is rounded to
     e4m3 times a power of two, the sums are f32, the result is rounded to f16 and
-    run through the op-graph."""
-    return _matmul_fp8(a, w, c, m, ep, False)
+    run through the op-graph. scratch: a device tensor of w.scratch_bytes(m) bytes, the
+    call's own until its work has run (a captured call's as long as its graph);
+    without one the library has it, a captured call's until the process ends."""
+    return _matmul_fp8(a, w, c, m, ep, False, scratch)
 
 
-def matmul_fp8(a, w: Fp8Weights, c, m: int):
-    return _matmul_fp8(a, w, c, m, None, False)
+def matmul_fp8(a, w: Fp8Weights, c, m: int, scratch=None):
+    return _matmul_fp8(a, w, c, m, None, False, scratch)
 
 
-def matmul_fp8_bf16_ep(a, w: Fp8Weights, c, m: int, ep: Epilogue):
+def matmul_fp8_bf16_ep(a, w: Fp8Weights, c, m: int, ep: Epilogue, scratch=None):
     """matmul_fp8_ep over bf16 values."""
-    return _matmul_fp8(a, w, c, m, ep, True)
+    return _matmul_fp8(a, w, c, m, ep, True, scratch)
 
 
-def matmul_fp8_bf16(a, w: Fp8Weights, c, m: int):
-    return _matmul_fp8(a, w, c, m, None, True)
+def matmul_fp8_bf16(a, w: Fp8Weights, c, m: int, scratch=None):
+    return _matmul_fp8(a, w, c, m, None, True, scratch)
 
 
 def q4_chained(a, w: Q4Weights, c, ep: Epilogue | None = None, done=None, ready=None, *, m: int = 1,
@@ -1703,17 +1733,23 @@ class Experts:
     def device(self) -> int:
         return self._on
 
-    def forward(self, x, ids, weights, out, rows: int):
+    def scratch_bytes(self, rows: int, top_k: int) -> int:
+        """The scratch of a call of rows x top_k assignments."""
+        b = SZ()
+        _check(lib().smg_experts_scratch_bytes(self._h, rows, top_k, C.byref(b)), "smg_experts_scratch_bytes")
+        return b.value
+
+    def forward(self, x, ids, weights, out, rows: int, scratch=None):
         """out (rows x width, of x's type: f16, or bf16 tensors; it may be x) = the
         weighted sums. ids int32 and weights float32, rows x top_k each. Host arrays or device
-        tensors."""
-        return self._run("forward", x, ids, weights, out, rows)
+        tensors. scratch: as matmul_fp8_ep's, of scratch_bytes(rows, top_k) bytes."""
+        return self._run("forward", x, ids, weights, out, rows, scratch)
 
-    def accumulate(self, x, ids, weights, y, rows: int):
+    def accumulate(self, x, ids, weights, y, rows: int, scratch=None):
         """y (float32, rows x width) += the weighted sums."""
-        return self._run("accumulate", x, ids, weights, y, rows)
+        return self._run("accumulate", x, ids, weights, y, rows, scratch)
 
-    def _run(self, what, x, ids, weights, out, rows):
+    def _run(self, what, x, ids, weights, out, rows, scratch):
         n = rows * self._d
         add = what == "accumulate"
         if _is_dev(x) and _is_dev(ids) and _is_dev(weights) and _is_dev(out):
@@ -1722,8 +1758,10 @@ class Experts:
             if (t in _T16 if _T16 else _torch16(False) and t in _T16) and count and rows > 0 and count % rows == 0 and (
                     _is_devn(x, n, on, t) and _is_devn(ids, count, on, i32) and _is_devn(weights, count, on, f32)
                     and _is_devn(out, n, on, f32 if add else t)):
-                return self._run_dev(add, x, ids, weights, out, rows, count // rows)
+                return self._run_dev(add, x, ids, weights, out, rows, count // rows, scratch)
         if not _same_side(x, ids, weights, out):
+            if scratch is not None:
+                raise TypeError("scratch belongs to calls of device tensors")
             xh = _host_x16(x, n, "x (rows*width)")
             if not isinstance(ids, np.ndarray) or ids.dtype != np.int32:
                 raise TypeError("ids: expected an int32 numpy array")
@@ -1743,12 +1781,16 @@ class Experts:
         top_k = self._top_k(ids.numel(), rows)
         _devn(weights, ids.numel(), "weights (rows*top_k)", self._on, torch.float32)
         _devn(out, n, "y (rows*width)" if add else "out (rows*width)", self._on, torch.float32 if add else x.dtype)
-        return self._run_dev(add, x, ids, weights, out, rows, top_k)
+        return self._run_dev(add, x, ids, weights, out, rows, top_k, scratch)
 
-    def _run_dev(self, add, x, ids, weights, out, rows, top_k):
-        fn = _lib.smg_experts_accumulate_dev if add else _lib.smg_experts_forward_dev
+    def _run_dev(self, add, x, ids, weights, out, rows, top_k, scratch):
+        if scratch is None:
+            fn, own = _lib.smg_experts_accumulate_dev if add else _lib.smg_experts_forward_dev, ()
+        else:
+            fn = _lib.smg_experts_accumulate_ws_dev if add else _lib.smg_experts_forward_ws_dev
+            own = _own_scratch(scratch, self._on)
         rc = fn(self._h, x.data_ptr(), x.dtype is _torch16(True), ids.data_ptr(), weights.data_ptr(), rows, top_k,
-                out.data_ptr(), _stream_on(self._on))
+                out.data_ptr(), *own, _stream_on(self._on))
         if rc:
             _check(rc, "Experts.accumulate" if add else "Experts.forward")
         return out
