@@ -110,8 +110,8 @@ __device__ __forceinline__ float4_t fp8_mfma_f16(const int8x_t &w, const half8_t
 
 // A hidden value act(g) u, act silu or the tanh form of gelu: g / (1 + e^-y) by the
 // hardware's 2^x and reciprocal (2^-23 each). past: e^-y is beyond 2^100 or so, and the
-// value is glu_far's: g e^y, its power in two halves, as the whole one may be too small
-// for an f32. (An f64 branch for each of a lane's values instead cost the products of few
+// value is glu_far's: g e^y u, a half of the power with either factor, as g e^y alone may
+// be too small for an f32 where u is large. (An f64 branch for each of a lane's values instead cost the products of few
 // rows a sixth of their time, in registers: 296 assignments of 4096 to 1792, 324 us
 // against 277.)
 __device__ __forceinline__ float glu_power(bool gelu, float g) {  // -log2 of e^y
@@ -124,7 +124,7 @@ __device__ __forceinline__ float glu_near(bool gelu, float g, float u, bool &pas
 }
 __device__ __forceinline__ float glu_far(bool gelu, float g, float u) {
     const float h = __builtin_amdgcn_exp2f(-0.5f * glu_power(gelu, g));
-    return g * h * h * u;
+    return (g * h) * (h * u);
 }
 
 // acc += part * sw, the weight block's scale: one f32 rounding an element.

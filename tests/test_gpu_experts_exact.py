@@ -186,3 +186,40 @@ def test_hidden_values_keep_their_codes(smg, rows, bf16):
     for g in got:
         err = np.linalg.norm(g - want) / np.linalg.norm(want)
         assert err < 2.0 ** -10, err
+
+
+@pytest.mark.parametrize("gelu", [False, True])
+@pytest.mark.parametrize("rows", [1, 3, 60, 500])
+def test_gates_whose_power_is_no_f32(smg, rows, gelu):
+    """Gates of -72 .. -120 (gelu: -8 .. -12), where g / (1 + e^-y) lies below f32's normal
+    range, times up values that bring it back: the second product is the identity, so the
+    outputs are the hidden values' codes, those within 2^-10 of a border aside (the hardware's
+    2^x of arguments up to 2^8 is off by 2^-15)."""
+    rng = np.random.default_rng(rows)
+    n, gates = 128, -np.float64(np.arange(8, 13) if gelu else np.arange(72, 121, 8))
+    experts = len(gates)
+    y = 2 * 0.7978845608028654 * (gates + 0.044715 * gates ** 3) if gelu else gates
+    up = rng.choice(ref.VALUES[0x38:0x58], (experts, n, n))  # 1 .. 15
+    h = (gates * np.exp(y) / (1 + np.exp(y)))[:, None, None] * up * 2.0 ** 100
+    back = 2.0 ** -np.round(np.log2(np.abs(h).max((1, 2)) / 64))
+    ones = np.ones((experts, 1, 1))
+    gate = np.broadcast_to(exact.code_of(gates)[:, None, None], (experts, n, n))
+    e = smg.Experts(gate, np.float32(ones), exact.code_of(up), np.float32(ones * 2.0 ** 100),
+                    np.broadcast_to(np.where(np.eye(n, dtype=bool), 0x38, 0).astype(np.uint8), (experts, n, n)),
+                    np.float32(ones * back[:, None, None]), experts, n, n, smg.Gate.Gelu if gelu else smg.Gate.Silu)
+    at, ids = rng.integers(0, n, rows), rng.integers(0, experts, (rows, 1)).astype(np.int32)
+    x = np.zeros((rows, n))
+    x[np.arange(rows), at] = 1
+    hr = h[ids[:, 0], :, at]
+    want = ref.quantize_rows(hr)
+    clear = (ref.quantize_rows(hr * (1 + 2.0 ** -10)) == want) & (ref.quantize_rows(hr * (1 - 2.0 ** -10)) == want)
+    # (a whole row's exponent changes with its largest value)
+    clear &= clear[np.arange(rows), np.abs(hr).argmax(1)][:, None]
+    assert clear.mean() > 0.8
+    want *= back[ids]
+    for bf16 in (False, True):
+        b, w = bits(x, bf16), np.ones((rows, 1), np.float32)
+        got = values(run_experts(e, b, ids, w, bf16), bf16)
+        acc = accumulate(e, b, ids, w, np.zeros((rows, n), np.float32), bf16)
+        for g in (got, acc):
+            assert np.array_equal(g[clear], want[clear]), (np.argwhere(clear & (g != want))[0], (clear & (g != want)).sum())
