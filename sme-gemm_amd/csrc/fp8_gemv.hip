@@ -11,6 +11,8 @@
 // pass first and multiplied in the same way (fp8_gemv_rows).
 // What bounds it: reading the weights once (one row, weights from HBM: 16.8 MB of a 4096 x
 // 4096 layer in 5.1 us, 58.7 MB of 14336 x 4096 in 11.4, 5.1 TB/s).
+#include <algorithm>
+
 #include "fp8_core.cuh"
 
 namespace smg {
@@ -187,10 +189,10 @@ __global__ void __launch_bounds__(256) fp8_quant(const uint16_t *x, uint32_t row
     if (lg == 0) e[(((size_t)mt / 4 * nkb + kb) * 16 + lr) * 4 + mt % 4] = (uint8_t)eb;
 }
 
-// A thread 16 bytes of the fragment order.
+// A thread 16 bytes of the fragment order, from number `first` on.
 __global__ void __launch_bounds__(256) fp8_pack(const uint8_t *src, uint8_t *dst, uint32_t n, uint32_t k, uint32_t n16,
-                                                uint32_t nkb, size_t chunks) {
-    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
+                                                uint32_t nkb, size_t first, size_t chunks) {
+    const size_t i = first + (size_t)blockIdx.x * 256 + threadIdx.x;
     if (i >= chunks) return;
     const uint32_t lane = i % 64, half = i / 64 % 2;
     const size_t frag = i / 128;
@@ -218,10 +220,15 @@ __global__ void __launch_bounds__(256) fp8_pack(const uint8_t *src, uint8_t *dst
 
 hipError_t launch_fp8_pack(const Fp8Mat &w, const uint8_t *src, uint8_t *codes, hipStream_t s) {
     const size_t chunks = w.code_bytes() * w.mats / 16;
-    if (chunks == 0) return hipSuccess;
-    hipLaunchKernelGGL(fp8_pack, dim3((uint32_t)((chunks + 255) / 256)), dim3(256), 0, s, src, codes, w.n, w.k, w.n16, w.nkb,
-                       chunks);
-    return hipGetLastError();
+    // (a launch of 2^32 threads or more runs their number modulo 2^32, without an error)
+    constexpr size_t PIECE = (size_t)1 << 31;
+    for (size_t first = 0; first < chunks; first += PIECE) {
+        const size_t blocks = (std::min(chunks - first, PIECE) + 255) / 256;
+        hipLaunchKernelGGL(fp8_pack, dim3((uint32_t)blocks), dim3(256), 0, s, src, codes, w.n, w.k, w.n16, w.nkb, first, chunks);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 static bool rows_vec(const uint16_t *x, size_t k) { return k % 8 == 0 && ((uintptr_t)x & 15) == 0; }
