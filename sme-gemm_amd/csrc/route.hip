@@ -316,7 +316,7 @@ __global__ void __launch_bounds__(RT_NT) route(RouteArgs a) {
 }
 
 template <int TYPE>
-hipError_t launch_type(const RouteArgs &a, hipStream_t s) {
+hipError_t launch_rows(const RouteArgs &a, hipStream_t s) {
     const bool quarter = a.experts <= 256 && a.top_k < 16;  // 16 lanes a row
     const uint32_t per = RT_W * (quarter ? 4 : 1);
     const dim3 grid((a.rows + per - 1) / per), block(RT_NT);
@@ -330,6 +330,20 @@ hipError_t launch_type(const RouteArgs &a, hipStream_t s) {
         else hipLaunchKernelGGL((route<TYPE, 16, 64>), grid, block, 0, s, a);
     }
     return hipGetLastError();
+}
+// (a launch of 2^32 threads or more runs their number modulo 2^32, without an error)
+template <int TYPE>
+hipError_t launch_type(RouteArgs a, hipStream_t s) {
+    constexpr uint32_t PIECE = 1u << 24;  // rows
+    for (uint32_t left = a.rows; left != 0; left -= a.rows) {
+        a.rows = left < PIECE ? left : PIECE;
+        const hipError_t e = launch_rows<TYPE>(a, s);
+        if (e != hipSuccess) return e;
+        a.logits = (const uint8_t *)a.logits + (size_t)a.rows * a.experts * (TYPE == LOGIT_F32 ? 4 : 2);
+        a.ids += (size_t)a.rows * a.top_k;
+        a.weights += (size_t)a.rows * a.top_k;
+    }
+    return hipSuccess;
 }
 
 }  // namespace
