@@ -533,18 +533,23 @@ __global__ void __launch_bounds__(256) experts_sum(const float *part, const int3
     }
     for (uint32_t c = 0; c < ne; c++) out[o + c] = from_f32<BF16>(s[c]);
 }
+// Threads of a launch over rows: one of 2^32 or more runs their number modulo 2^32, without
+// an error.
+constexpr size_t MOST_THREADS = (size_t)1 << 31;
 template <bool BF16>
 hipError_t launch_sum(const ExpertCall &c, const float *part, const int32_t *place, uint32_t experts, uint32_t d,
                       hipStream_t s) {
-    const uint32_t parts = (d + 2047) / 2048;
-    const dim3 grid(c.rows * parts);
-    if (d % 8 == 0)
-        hipLaunchKernelGGL((experts_sum<BF16, true>), grid, dim3(256), 0, s, part, place, c.ids, c.weights, c.top_k, experts, d,
-                           parts, c.out, c.y);
-    else
-        hipLaunchKernelGGL((experts_sum<BF16, false>), grid, dim3(256), 0, s, part, place, c.ids, c.weights, c.top_k, experts, d,
-                           parts, c.out, c.y);
-    return hipGetLastError();
+    const uint32_t parts = (d + 2047) / 2048, piece = (uint32_t)(MOST_THREADS / 256 / parts);
+    for (uint32_t r0 = 0; r0 < c.rows; r0 += piece) {
+        const size_t as = (size_t)r0 * c.top_k, o = (size_t)r0 * d;
+        const dim3 grid(std::min(piece, c.rows - r0) * parts);
+        hipLaunchKernelGGL((d % 8 == 0 ? experts_sum<BF16, true> : experts_sum<BF16, false>), grid, dim3(256), 0, s,
+                           place ? part : part + as * d, place ? place + as : nullptr, c.ids + as, c.weights + as, c.top_k,
+                           experts, d, parts, c.out ? c.out + o : nullptr, c.y ? c.y + o : nullptr);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 // The plan, by one workgroup: the experts' counts, their rows' starts, the tiles, and
@@ -739,9 +744,14 @@ hipError_t launch_experts(const ExpertSet &e, const ExpertCall &c, void *scratch
     const uint16_t *x = l.padded ? l.padded : c.x;
     hipError_t err;
     if (l.padded) {
-        const size_t blocks = ((size_t)c.rows * (xld / 8) + 255) / 256;
-        hipLaunchKernelGGL(pad_rows, dim3((uint32_t)blocks), dim3(256), 0, s, c.x, c.rows, d, xld, l.padded);
-        if ((err = hipGetLastError()) != hipSuccess) return err;
+        const uint32_t piece = (uint32_t)(MOST_THREADS / (xld / 8));
+        for (uint32_t r0 = 0; r0 < c.rows; r0 += piece) {
+            const uint32_t n = std::min(piece, c.rows - r0);
+            const size_t blocks = ((size_t)n * (xld / 8) + 255) / 256;
+            hipLaunchKernelGGL(pad_rows, dim3((uint32_t)blocks), dim3(256), 0, s, c.x + (size_t)r0 * d, n, d, xld,
+                               l.padded + (size_t)r0 * xld);
+            if ((err = hipGetLastError()) != hipSuccess) return err;
+        }
     }
     if (l.hidden) {
         EgArgs g = {};

@@ -1,6 +1,10 @@
 """Calls of so many rows that a launch of a thread, or a few, for each would pass 2^32 threads
 (such a launch runs their number modulo 2^32, without an error)."""
+import numpy as np
 import pytest
+
+from test_gpu_experts import build, random_experts, run_experts
+from test_gpu_fp8 import bits, dev16
 
 pytestmark = pytest.mark.gpu
 
@@ -28,3 +32,23 @@ def test_routing(smg, rows, experts, top_k):
         want = torch.sort(l, dim=1, descending=True, stable=True)
         assert torch.equal(ids[at:at + 1000], want.indices[:, :top_k].int())
         assert torch.allclose(w[at:at + 1000], torch.softmax(want.values[:, :top_k], 1), rtol=1e-5, atol=0)
+
+
+@pytest.mark.parametrize("d", [16, 15])
+def test_experts(smg, d):
+    """Rows of a few kinds: equal rows give equal bits, to the last."""
+    import torch
+    room(40 << 30)
+    rng = np.random.default_rng(d)
+    rows, experts, ffn, kinds = 2 ** 24 + 3, 2, 16, 7
+    e = build(smg, random_experts(rng, experts, d, ffn), experts, d, ffn)
+    few = bits(rng.standard_normal((kinds, d)), True)
+    ids, w = rng.integers(0, experts, (kinds, 1)).astype(np.int32), rng.uniform(0.1, 1, (kinds, 1)).astype(np.float32)
+    many = 200  # (the tiles' form, as the long call's)
+    at = np.arange(kinds * many) // many
+    want = run_experts(e, few[at], ids[at], w[at], True)[::many]
+    kind = torch.arange(rows, device="cuda") % kinds
+    x = dev16(few, True)[kind]
+    out = torch.full((rows, d), float("nan"), dtype=torch.bfloat16, device="cuda")
+    e.forward(x, torch.from_numpy(ids).cuda()[kind], torch.from_numpy(w).cuda()[kind], out, rows)
+    assert torch.equal(out, dev16(want, True)[kind])
