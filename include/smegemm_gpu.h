@@ -163,7 +163,7 @@ int smg_q1_quantize(const float *w, int layout, size_t n, size_t k, size_t block
 /* 8-bit floating-point weights (no reference counterpart): e4m3 codes
  * codes[j*k + d] of n columns and k depths, and an f32 scale for each block of
  * 128 columns x 128 depths, scales[(j/128)*ceil(k/128) + d/128], as checkpoints
- * hold them; a weight is its code times its block's scale. k < 2^25, n < 2^30.
+ * hold them; a weight is its code times its block's scale. k < 2^25, n < 2^27.
  * _dev takes device arrays, read on `stream`, which it waits for. */
 int smg_fp8_create(const uint8_t *codes, const float *scales, size_t n, size_t k, smg_weights **out);
 int smg_fp8_create_dev(const uint8_t *codes, const float *scales, size_t n, size_t k, void *stream,

@@ -533,8 +533,7 @@ __global__ void __launch_bounds__(256) experts_sum(const float *part, const int3
     }
     for (uint32_t c = 0; c < ne; c++) out[o + c] = from_f32<BF16>(s[c]);
 }
-// Threads of a launch over rows: one of 2^32 or more runs their number modulo 2^32, without
-// an error.
+// Threads of a launch over rows (launchable).
 constexpr size_t MOST_THREADS = (size_t)1 << 31;
 template <bool BF16>
 hipError_t launch_sum(const ExpertCall &c, const float *part, const int32_t *place, uint32_t experts, uint32_t d,
@@ -797,7 +796,9 @@ hipError_t launch_experts(const ExpertSet &e, const ExpertCall &c, void *scratch
     hipLaunchKernelGGL(expert_plan, dim3(1), dim3(PL_NT), 0, s, c.ids, l.p);
     if ((err = hipGetLastError()) != hipSuccess) return err;
     const uint32_t nkb = e.gate.nkb;
-    const dim3 rows((uint32_t)(((size_t)l.p.max_rows / 16 * nkb + 3) / 4));
+    const size_t waves = (size_t)l.p.max_rows / 16 * nkb;
+    if (!launchable(waves, 64)) return hipErrorInvalidConfiguration;
+    const dim3 rows((uint32_t)((waves + 3) / 4));
     if (c.bf16) hipLaunchKernelGGL((expert_rows<true>), rows, dim3(256), 0, s, x, xld, l.p, d, nkb, l.x);
     else hipLaunchKernelGGL((expert_rows<false>), rows, dim3(256), 0, s, x, xld, l.p, d, nkb, l.x);
     if ((err = hipGetLastError()) != hipSuccess) return err;

@@ -1,6 +1,9 @@
 // Launch interface of the 8-bit floating-point products (fp8_gemv.hip,
 // fp8_gemm.hip). Internal to the library.
 //
+// Launches whose threads would pass 2^32 - 1 (which run their number modulo 2^32, without
+// an error) are refused with hipErrorInvalidConfiguration, or split.
+//
 // Weights are e4m3 codes with an f32 scale for each 128 x 128 block of a matrix
 // of n columns and k depths (a checkpoint's [n][k] codes and [n/128][k/128]
 // scales). On the device the codes are in the order the matrix instructions read
@@ -20,6 +23,7 @@ namespace smg {
 
 constexpr uint32_t FP8_BLOCK = 128;      // depths (and columns) of a scale
 constexpr uint32_t FP8_FRAG = 2048;      // bytes of 16 columns (rows) x 128 depths
+inline bool launchable(size_t blocks, size_t threads) { return blocks * threads < (size_t)1 << 32; }
 
 // One or several matrices of one shape (a mixture's experts), one after another.
 struct Fp8Mat {

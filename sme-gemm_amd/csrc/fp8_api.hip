@@ -14,8 +14,9 @@ using namespace smg;
 namespace {
 
 // Bounds within which a matrix's and a call's offsets stay in the kernels' types: a
-// column tile's fragments within 2^31 bytes (nkb <= 2^18), the grids within 2^31.
-constexpr size_t FP8_MAX_K = (size_t)1 << 25, FP8_MAX_N = (size_t)1 << 30;
+// column tile's fragments within 2^31 bytes (nkb <= 2^18), a launch's threads below 2^32 (the
+// products of few rows: 512 for 16 columns).
+constexpr size_t FP8_MAX_K = (size_t)1 << 25, FP8_MAX_N = (size_t)1 << 27;
 
 // No exception leaves a C entry.
 template <class F>
@@ -194,6 +195,7 @@ int experts_dev(const smg_experts *e, const uint16_t *x, int bf16, const int32_t
     CallScratch sc(e->device, stream, experts_scratch_bytes(set, c), own);
     if ((rc = sc.check("experts"))) return rc;
     const hipError_t err = launch_experts(set, c, sc.buf(), (hipStream_t)stream);
+    if (err == hipErrorInvalidConfiguration) return report(SMG_EINVAL, "too many rows a call");
     return err == hipSuccess ? SMG_OK : report_hip(SMG_EHIP, "experts", err);
 }
 
@@ -232,6 +234,7 @@ int fp8_dev(size_t m, const smg_weights *w, uint16_t *dst, const uint16_t *lhs, 
     if ((rc = sc.check("smg_fp8_matmul_dev"))) return rc;
     hipStream_t s = (hipStream_t)stream;
     hipError_t e = launch_fp8_matmul(w->f8, m, dst, lhs, p.fused, bf16 != 0, sc.buf(), s);
+    if (e == hipErrorInvalidConfiguration) return report(SMG_EINVAL, "too many rows a call");
     if (e == hipSuccess) e = run_graph_tail(p, dst, m, n, bf16 != 0, s);
     return e == hipSuccess ? SMG_OK : report_hip(SMG_EHIP, "smg_fp8_matmul_dev", e);
 }

@@ -678,9 +678,10 @@ uint32_t f8_full_tiles(size_t m, size_t n) {
 }
 template <bool BF16>
 hipError_t launch_f8_big(F8Args f, bool halves, const EpArgs &ep, int epv, hipStream_t s) {
-    const uint32_t nt = (f.d.n + 255) / 256, tiles = (f.d.m + 255) / 256 * nt;
+    const size_t nt = (f.d.n + 255) / 256, tiles = (f.d.m + (size_t)255) / 256 * nt;
+    if (!launchable(2 * tiles, 512)) return hipErrorInvalidConfiguration;
     f.full = halves ? 0 : f8_full_tiles(f.d.m, f.d.n);
-    const dim3 grid(f.full == 0 ? (f.d.m + 127) / 128 * nt : f.full + 2 * (tiles - f.full)), block(512);
+    const dim3 grid((uint32_t)(f.full == 0 ? (f.d.m + 127) / 128 * nt : f.full + 2 * (tiles - f.full))), block(512);
     switch (epv) {
     case 1: hipLaunchKernelGGL((fp8_big<BF16, 1, F8_DENSE>), grid, block, 0, s, f, ep); break;
     case 2: hipLaunchKernelGGL((fp8_big<BF16, 2, F8_DENSE>), grid, block, 0, s, f, ep); break;
@@ -692,7 +693,9 @@ hipError_t launch_f8_big(F8Args f, bool halves, const EpArgs &ep, int epv, hipSt
 
 template <int BM, int BN, int NSTG, bool BF16>
 hipError_t launch_f8_tile(const F8Args &f, const EpArgs &ep, int epv, hipStream_t s) {
-    const dim3 grid(((f.d.m + BM - 1) / BM) * ((f.d.n + BN - 1) / BN)), block(256);
+    const size_t tiles = (size_t)((f.d.m + BM - 1) / BM) * ((f.d.n + BN - 1) / BN);
+    if (!launchable(tiles, 256)) return hipErrorInvalidConfiguration;
+    const dim3 grid((uint32_t)tiles), block(256);
     switch (epv) {
     case 1: hipLaunchKernelGGL((fp8_tile<BM, BN, NSTG, BF16, 1>), grid, block, 0, s, f, ep); break;
     case 2: hipLaunchKernelGGL((fp8_tile<BM, BN, NSTG, BF16, 2>), grid, block, 0, s, f, ep); break;
@@ -799,8 +802,10 @@ hipError_t launch_fp8_grouped(const Fp8Mat &w, const Fp8Mat *up, uint32_t act, c
     f.head = p.head;
     f.tiles = p.tiles;
     const uint32_t cols = up ? 128 : 256;
-    const dim3 grid(p.max_tiles * (up && exact ? 2 : 1) * ((w.n + cols - 1) / cols)), block(512);
-    if (grid.x == 0) return hipSuccess;
+    const size_t tiles = (size_t)p.max_tiles * (up && exact ? 2 : 1) * ((w.n + cols - 1) / cols);
+    if (!launchable(tiles, 512)) return hipErrorInvalidConfiguration;
+    const dim3 grid((uint32_t)tiles), block(512);
+    if (tiles == 0) return hipSuccess;
     if (up) {
         f.w2 = up->codes;
         f.sw2 = up->scales;

@@ -220,7 +220,6 @@ __global__ void __launch_bounds__(256) fp8_pack(const uint8_t *src, uint8_t *dst
 
 hipError_t launch_fp8_pack(const Fp8Mat &w, const uint8_t *src, uint8_t *codes, hipStream_t s) {
     const size_t chunks = w.code_bytes() * w.mats / 16;
-    // (a launch of 2^32 threads or more runs their number modulo 2^32, without an error)
     constexpr size_t PIECE = (size_t)1 << 31;
     for (size_t first = 0; first < chunks; first += PIECE) {
         const size_t blocks = (std::min(chunks - first, PIECE) + 255) / 256;
@@ -237,6 +236,7 @@ hipError_t launch_fp8_quant(const uint16_t *x, size_t rows, size_t k, bool bf16,
     const uint32_t nkb = (uint32_t)((k + 127) / 128), waves = (uint32_t)((rows + 15) / 16) * nkb;
     if (waves == 0) return hipSuccess;
     const dim3 grid((waves + 3) / 4);
+    if (!launchable(grid.x, 256)) return hipErrorInvalidConfiguration;
 #define SMG_FP8_Q(B, V) hipLaunchKernelGGL((fp8_quant<B, V>), grid, dim3(256), 0, s, x, (uint32_t)rows, (uint32_t)k, nkb, out.q, out.e)
     if (rows_vec(x, k)) {
         if (bf16) SMG_FP8_Q(true, true);

@@ -331,7 +331,7 @@ hipError_t launch_rows(const RouteArgs &a, hipStream_t s) {
     }
     return hipGetLastError();
 }
-// (a launch of 2^32 threads or more runs their number modulo 2^32, without an error)
+// (as launchable asks)
 template <int TYPE>
 hipError_t launch_type(RouteArgs a, hipStream_t s) {
     constexpr uint32_t PIECE = 1u << 24;  // rows

@@ -52,3 +52,19 @@ def test_experts(smg, d):
     out = torch.full((rows, d), float("nan"), dtype=torch.bfloat16, device="cuda")
     e.forward(x, torch.from_numpy(ids).cuda()[kind], torch.from_numpy(w).cuda()[kind], out, rows)
     assert torch.equal(out, dev16(want, True)[kind])
+
+
+def test_products_of_too_many_tiles_are_refused(smg):
+    """2^30 rows of one column: 2^26 waves quantize them, 2^24 workgroups of 256 threads multiply."""
+    import torch
+    room(180 << 30)
+    m = 2 ** 30
+    w = smg.Fp8Weights(np.uint8([[0x38]]), np.float32([[1]]), 1, 1)
+    a, c = torch.ones(m, 1, device="cuda", dtype=torch.float16), torch.full((m, 1), 7.0, device="cuda", dtype=torch.float16)
+    scratch = torch.empty(w.scratch_bytes(m), dtype=torch.uint8, device="cuda")
+    with pytest.raises(smg.SmeGemmError, match="too many rows"):
+        smg.matmul_fp8(a, w, c, m, scratch=scratch)
+    torch.cuda.synchronize()
+    assert bool((c == 7).all())
+    smg.matmul_fp8(a[:m // 2], w, c[:m // 2], m // 2, scratch=scratch)
+    assert bool((c[:m // 2] == 1).all()) and bool((c[m // 2:] == 7).all())
