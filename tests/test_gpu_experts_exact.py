@@ -223,3 +223,36 @@ def test_gates_whose_power_is_no_f32(smg, rows, gelu):
         acc = accumulate(e, b, ids, w, np.zeros((rows, n), np.float32), bf16)
         for g in (got, acc):
             assert np.array_equal(g[clear], want[clear]), (np.argwhere(clear & (g != want))[0], (clear & (g != want)).sum())
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("rows", [1, 5, 40, 400])
+def test_nan_codes_and_rows(smg, rows, bf16):
+    """A NaN code of a gate or up matrix makes the rows of its expert NaN, one of a down matrix
+    that column of them; a NaN or infinite activation its row. Nothing else changes."""
+    rng = np.random.default_rng(rows)
+    experts, d, ffn, k = 6, 140, 136, 2
+    parts = exact.make(rng, experts, d, ffn)
+    xv, w = exact.rows_of(rng, rows, d), rng.uniform(0.1, 1, (rows, k)).astype(np.float32)
+    ids = np.stack([rng.permutation(experts)[:k] for _ in range(rows)]).astype(np.int32)
+    plain = build(smg, parts, experts, d, ffn)
+    want = [values(run_experts(plain, bits(xv, bf16), ids, w, bf16), bf16),
+            accumulate(plain, bits(xv, bf16), ids, w, np.zeros((rows, d), np.float32), bf16)]
+    for which, at in ((0, (1, 77, 3)), (1, (2, 135, 139)), (2, (3, 99, 130))):
+        bad = [tuple(np.copy(a) for a in p) for p in parts]
+        bad[which][0][at] = 0x7F if which else 0xFF
+        e = build(smg, bad, experts, d, ffn)
+        hit = np.zeros((rows, d), bool)
+        hit[(ids == at[0]).any(1), at[1] if which == 2 else slice(None)] = True
+        got = [values(run_experts(e, bits(xv, bf16), ids, w, bf16), bf16),
+               accumulate(e, bits(xv, bf16), ids, w, np.zeros((rows, d), np.float32), bf16)]
+        for g, x in zip(got, want):
+            assert np.array_equal(np.isnan(g), hit) and np.array_equal(g[~hit], x[~hit]), which
+    for v in (np.nan, np.inf, -np.inf):
+        x = xv.copy()
+        x[rows // 2, 133] = v
+        got = [values(run_experts(plain, bits(x, bf16), ids, w, bf16), bf16),
+               accumulate(plain, bits(x, bf16), ids, w, np.zeros((rows, d), np.float32), bf16)]
+        for g, y in zip(got, want):
+            hit = np.arange(rows) == rows // 2
+            assert np.isnan(g[hit]).all() and np.array_equal(g[~hit], y[~hit])
