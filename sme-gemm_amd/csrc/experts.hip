@@ -18,7 +18,7 @@
 // What bounds it: few rows, reading the weights of the experts that are used; many
 // rows, the products. Measured (weights from memory): one row, 6 of 64 experts, 2048 to 1280
 // 14.5 us (47 MB); 37 rows, 8 of 64, 4096 to 1792 270 us (1.39 GB, 5.1 TB/s); 3001 rows, 8 of
-// 128, 2048 to 1000 532 us (f16); 2048 rows, 2 of 8, 4096 to 14336 892 us (bf16; 1.6 PFLOP/s).
+// 128, 2048 to 1000 527 us (f16); 2048 rows, 2 of 8, 4096 to 14336 854 us (bf16; 1.7 PFLOP/s).
 #include <algorithm>
 
 #include "experts.h"
@@ -42,7 +42,7 @@ struct EgArgs {
     const float *weights;
     uint16_t *out;
     float *y;
-    uint32_t rows, top_k, assignments, experts, d, xld, hld, act;  // xld: x's rows
+    uint32_t top_k, assignments, experts, d, xld, hld, act;  // xld: x's rows
 };
 
 // The expert of slot y and the assignments that chose it: with no more assignments
@@ -765,7 +765,6 @@ hipError_t launch_experts(const ExpertSet &e, const ExpertCall &c, void *scratch
         g.weights = c.weights;
         g.out = c.out;
         g.y = c.y;
-        g.rows = c.rows;
         g.top_k = c.top_k;
         g.assignments = as;
         g.experts = experts;

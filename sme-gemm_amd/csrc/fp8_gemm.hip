@@ -708,9 +708,6 @@ hipError_t launch_f8_tile(const F8Args &f, const EpArgs &ep, int epv, hipStream_
 // The tile for an m x n x k product: the least of a cost in us, steps of 128 depths x
 // (full rounds of the compute units x occupancy, each at `full`, and a last round that
 // grows from `one` to `full`) + `fixed`, the constants measured on 256 compute units
-// The tile for an m x n x k product: the least of a cost in us, steps of 128 depths x
-// (full rounds of the compute units x occupancy, each at `full`, and a last round that
-// grows from `one` to `full`) + `fixed`, the constants measured on 256 compute units
 // (large grids draw the clock down, so `full` is also what the power allows). Measured
 // (us with the rows' quantization, bf16, weights from memory, tiles of 256 rows ended by
 // halves / 128x256 / 64x128 / 64x64): 4096 x 14336 x 4096 241 / 279 / 361 / 431; 2048 x
