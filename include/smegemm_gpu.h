@@ -342,7 +342,8 @@ int smg_fp8_matmul_dev(size_t m, const smg_weights *w, uint16_t *dst, const uint
                        int bf16, void *stream);
 /* smg_fp8_matmul_dev in the caller's scratch: `bytes` of device memory at a multiple of
  * 256, at least smg_fp8_scratch_bytes' (which may be 0, scratch NULL), that nothing else
- * uses until the call's work has run, or as long as a graph holds it. */
+ * uses until the call's work has run, or as long as a graph holds it. (The library's own
+ * for eager calls is 64 GiB at most, over all streams; SMG_ENOMEM past that.) */
 int smg_fp8_scratch_bytes(const smg_weights *w, size_t m, size_t *bytes);
 int smg_fp8_matmul_ws_dev(size_t m, const smg_weights *w, uint16_t *dst, const uint16_t *lhs, const ep_desc16 *ep,
                           int bf16, void *scratch, size_t bytes, void *stream);

@@ -98,9 +98,10 @@ __device__ __forceinline__ half8_t fp8_to_f16(uint32_t a, uint32_t b) {
     const half2_t x = fp8_pair_f16(a, false), y = fp8_pair_f16(a, true), z = fp8_pair_f16(b, false), w = fp8_pair_f16(b, true);
     return (half8_t){x[0], x[1], y[0], y[1], z[0], z[1], w[0], w[1]};
 }
-// The codes' sums of a fragment by f16 products, which drop nothing of them, at a quarter
-// of the rate: for kernels that wait for memory and whose results are rounded to codes
-// again (where a sum a little off may cross the border of two).
+// The codes' sums of a fragment by f16 products, which drop nothing of them (2^-27 of a sum's
+// 2-norm on the same data), at half the rate and after widening: for kernels that wait for
+// memory and whose results are rounded to codes again (where a sum a little off may cross
+// the border of two).
 __device__ __forceinline__ float4_t fp8_mfma_f16(const int8x_t &w, const half8_t (&a)[4]) {
     float4_t c = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
