@@ -8,6 +8,17 @@ from test_gpu_fp8 import check, host16, values
 pytestmark = pytest.mark.gpu
 
 
+@pytest.fixture(autouse=True)
+def give_back():
+    """What these tests took does not stay in torch's cache."""
+    yield
+    import gc
+
+    import torch
+    gc.collect()
+    torch.cuda.empty_cache()
+
+
 def test_weights_past_64_gib(smg):
     import torch
     n, k = 65664, 1 << 20

@@ -9,6 +9,17 @@ from test_gpu_fp8 import bits, dev16
 pytestmark = pytest.mark.gpu
 
 
+@pytest.fixture(autouse=True)
+def give_back():
+    """What these tests took does not stay in torch's cache."""
+    yield
+    import gc
+
+    import torch
+    gc.collect()
+    torch.cuda.empty_cache()
+
+
 def room(n):
     import torch
     torch.cuda.empty_cache()
